@@ -19,15 +19,9 @@
 
 #include "ft_adam.h"
 #include "ft_types.hpp"
+#include "ft_vec.hpp"
 
 namespace ftk {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWave = 64;
 
@@ -65,35 +59,6 @@ __device__ __forceinline__ void adam_unit(f32x4& p, const f32x4& g, f32x4& m, f3
         m[k] = mk;
         v[k] = vk;
     }
-}
-
-// ---- 16-bit <-> 32-bit helpers ------------------------------------------------------------
-template <int DT>
-__device__ __forceinline__ float half_to_float(uint32_t bits16);
-template <>
-__device__ __forceinline__ float half_to_float<FT_BF16>(uint32_t b)
-{
-    return __builtin_bit_cast(float, b << 16);
-}
-template <>
-__device__ __forceinline__ float half_to_float<FT_F16>(uint32_t b)
-{
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)b);
-}
-
-template <int DT>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<FT_BF16>(float lo, float hi)
-{
-    f32x2 x = {lo, hi};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<FT_F16>(float lo, float hi)
-{
-    f32x2 x = {lo, hi};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
 }
 
 template <bool NT, typename T>

@@ -11,28 +11,12 @@
 #include <thread>
 #include <vector>
 
+#include "ft_counter.hpp"
 #include "ft_internal.hpp"
 
 namespace {
 
-#define FT_HD __host__ __device__ __forceinline__
-
-FT_HD uint64_t mix64(uint64_t z)  // the splitmix64 finaliser
-{
-    z ^= z >> 30;
-    z *= 0xbf58476d1ce4e5b9ull;
-    z ^= z >> 27;
-    z *= 0x94d049bb133111ebull;
-    z ^= z >> 31;
-    return z;
-}
-
-// 64 random bits of element `index` of `substream` under `seed`.
-FT_HD uint64_t element_bits(uint64_t seed, uint32_t substream, uint64_t index)
-{
-    const uint64_t key = mix64(seed ^ (0x9e3779b97f4a7c15ull * (static_cast<uint64_t>(substream) + 1u)));
-    return mix64(key + 0xd1342543de82ef95ull * index);
-}
+using ftc::element_bits;
 
 FT_HD float bits_as_float(uint32_t b)
 {
