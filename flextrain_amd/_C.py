@@ -29,6 +29,27 @@ class AdamSegment(ctypes.Structure):
     ]
 
 
+class Tokens(ctypes.Structure):
+    """Mirror of ``ft_tokens_t``: the token ids of one call."""
+
+    _fields_ = [
+        ("ids", c_void_p), ("outer", c_size_t), ("inner", c_size_t), ("outer_stride", c_size_t), ("inner_stride", c_size_t),
+        ("first_row", ctypes.c_int64), ("padding", ctypes.c_int64), ("id_bytes", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class Dropout(ctypes.Structure):
+    """Mirror of ``ft_dropout_t``: the mask of one call."""
+
+    _fields_ = [
+        ("p", c_double), ("seed", c_uint64), ("seed_dev", c_void_p), ("first_index", c_uint64), ("substream", c_uint32),
+        ("reserved", c_uint32),
+    ]
+
+
+NO_PADDING = -(1 << 63)
+
+
 class LinkProbe(ctypes.Structure):
     """Mirror of ``ft_link_probe_t`` (GB/s; ``both_*`` is the sum of the two directions)."""
 
@@ -82,6 +103,13 @@ EXPORTS = {
     "ft_link_bandwidth": (c_int, [c_size_t, c_int, c_int, POINTER(c_double)]),
     "ft_synth_fill": (c_int, [c_void_p, c_int, c_size_t, c_uint64, c_uint32, c_uint64, c_int, c_float, c_void_p]),
     "ft_synth_fill_host": (c_int, [c_void_p, c_int, c_size_t, c_uint64, c_uint32, c_uint64, c_int, c_float]),
+    "ft_embedding_lookup": (c_int, [POINTER(Tokens), c_void_p, c_int, c_size_t, c_size_t, c_void_p, c_int, c_size_t, c_size_t, c_double,
+                                    POINTER(Dropout), c_void_p]),
+    "ft_embedding_grad_workspace_bytes": (c_size_t, [c_size_t, c_size_t, c_size_t]),
+    "ft_embedding_grad": (c_int, [POINTER(Tokens), c_void_p, c_int, c_size_t, c_void_p, c_int, c_size_t, c_size_t, c_size_t, c_double,
+                                  c_int, POINTER(Dropout), c_void_p, c_size_t, c_void_p]),
+    "ft_dropout": (c_int, [c_void_p, c_int, c_size_t, c_void_p, c_size_t, c_void_p, c_int, c_size_t, c_size_t, c_size_t,
+                           POINTER(Dropout), c_void_p]),
     "ft_set_launch_tuning": (c_int, [c_int, c_int]),
     "ft_set_cache_tuning": (c_int, [c_size_t]),
     "ft_set_stats_launches": (c_int, [c_int]),

@@ -6,10 +6,13 @@ Importing the package does not touch the GPU; the native library is loaded on fi
 absence is an error (there is no CPU fallback).
 """
 from .adam import FlexTrainAdam, FlexTrainCPUAdam
+from .dropout_mask import dropout
+from .embedding_rows import embedding, embedding_grad_, embedding_lookup
 from .optimizer import PARAMS_KEY, STEP_KEY, FlexTrainCPUOptimizer, FlexTrainOptimizer
 from .param_group import GroupSegment, StepContext, StepContextContainer
 
 __all__ = [
     "FlexTrainAdam", "FlexTrainCPUAdam", "FlexTrainCPUOptimizer", "FlexTrainOptimizer",
     "GroupSegment", "StepContext", "StepContextContainer", "STEP_KEY", "PARAMS_KEY",
+    "dropout", "embedding", "embedding_grad_", "embedding_lookup",
 ]

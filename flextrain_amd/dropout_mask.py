@@ -1,0 +1,77 @@
+"""Dropout whose mask is never stored.
+
+Element ``i`` (row-major over the tensor's shape) stays or goes by a pure function of
+``(seed, substream, first_index + i)``: the counter generator of ``flextrain_amd.synth``, 48 bits per
+element, the same for every type, layout and split of a tensor. The backward pass makes the mask again
+instead of reading it. Give every call of a step its own ``substream`` (or range of indices) and every
+step its own ``seed``.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import _C
+from .rows import Seed, dropout_record, on_device, require_gpu, row_stride, with_even_rows
+
+
+def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index: int = 0, residual: Optional[Tensor] = None,
+            out: Optional[Tensor] = None) -> Tensor:
+    """``[residual +] keep * x / (1 - p)``, differentiable in ``x`` and ``residual``.
+
+    ``x``: fp32 / fp16 / bf16 GPU tensor whose rows (last dimension) lie at one distance. ``residual``
+    has x's shape; its type is the result's (without one, x's is). ``seed``: a number, or one int64
+    element of GPU memory -- then a pass recorded into a HIP graph follows a seed that changes between
+    replays; it must keep its value until the backward pass has run. ``out`` (no gradients then) may be
+    ``x`` or ``residual``. A dropped element contributes 0 even where ``x`` is inf or nan.
+    """
+    if out is None and torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, float(p), seed, substream, first_index, seed if isinstance(seed, Tensor) else None)
+    if out is not None and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, out)):
+        raise ValueError("out: not for tensors that require gradients")
+    return _apply(x, float(p), seed, substream, first_index, residual, out)
+
+
+def _apply(x: Tensor, p: float, seed: Seed, substream: int, first_index: int, residual: Optional[Tensor] = None, out: Optional[Tensor] = None,
+           dtype: Optional[torch.dtype] = None) -> Tensor:
+    require_gpu(x.device, x=x, residual=residual, out=out)
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
+    if dtype is None:
+        dtype = x.dtype if residual is None else residual.dtype
+    if out is None:
+        out = torch.empty(x.shape, dtype=dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != dtype:
+        raise ValueError(f"out must have shape {tuple(x.shape)} and type {dtype}")
+    cols = x.shape[-1] if x.dim() else 1
+    rows = x.numel() // cols if cols else 0
+    record = dropout_record(x.device, p, seed, substream, first_index)
+    with on_device(x.device):
+        _C.check("ft_dropout", _C.lib().ft_dropout(
+            x.data_ptr(), _C.dtype_code(x.dtype), row_stride("x", x, cols),
+            None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride("residual", residual, cols),
+            out.data_ptr(), _C.dtype_code(dtype), row_stride("out", out, cols), rows, cols, ctypes.byref(record),
+            _C.current_stream_ptr(x.device)))
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, substream, first_index, seed_tensor):
+        ctx.save_for_backward(seed_tensor)  # a seed that changes before the backward pass is found out
+        ctx.mask = (p, seed, substream, first_index)
+        ctx.x_dtype = x.dtype
+        return _apply(x, p, seed, substream, first_index, residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (seed_tensor,) = ctx.saved_tensors
+        p, seed, substream, first_index = ctx.mask
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = _apply(with_even_rows(dy), p, seed if seed_tensor is None else seed_tensor, substream, first_index, dtype=ctx.x_dtype)
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None

@@ -288,9 +288,11 @@ class FlexTrainOptimizer:
                 acc_views[i] += grad.flatten()
             return hook
 
+        self._param_offsets: Dict[Tensor, int] = {}
         offset = 0
         for i, param in enumerate(non_layerwise_params):
             end = offset + param.numel()
+            self._param_offsets[param] = offset
             self.non_layerwise_master_params.append(torch.nn.Parameter(self._master_para[offset:end]))
             param.grad = self._device_grad[offset:end].view_as(param)
             if self._gradacc_dtype_incompatible:
@@ -325,6 +327,23 @@ class FlexTrainOptimizer:
     @property
     def non_layerwise_numel(self) -> int:
         return self._device_para.numel()
+
+    def gradient_of(self, param: Tensor) -> Tensor:
+        """The part of the flat gradient buffer that the next step reads for ``param`` (in the type
+        gradients are accumulated in), in the shape of ``param``."""
+        if param not in self._param_offsets:
+            raise ValueError("not one of the parameters that this optimizer steps itself")
+        offset = self._param_offsets[param]
+        return self._step_grad[offset:offset + param.numel()].view(param.shape)
+
+    def embedding(self, tokens: Tensor, param: Tensor, **options) -> Tensor:
+        """``flextrain_amd.embedding`` of a table that this optimizer steps: the backward pass adds the
+        gradient straight into the buffer the step reads, only in the rows that a token names. Without
+        it, every micro-batch makes a dense gradient of the whole table and adds that (in a wider type
+        through a hook, reference ``flextrain/optimizer.py:194-215``). ``options``: those of
+        ``flextrain_amd.embedding`` except ``grad_into``."""
+        from .embedding_rows import embedding  # local import: keeps module load light
+        return embedding(tokens, param, grad_into=self.gradient_of(param), **options)
 
     def step(self, *args, **kwargs):
         """Steps the non-layerwise parameters (reference ``flextrain/optimizer.py:244-263``).

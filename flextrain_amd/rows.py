@@ -1,0 +1,99 @@
+"""What the row operators (embedding, dropout) share: argument checks and the C structs they fill."""
+from __future__ import annotations
+
+from contextlib import nullcontext
+from typing import Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from . import _C
+
+#: a seed by value, or one int64 element of GPU memory that the kernels read
+Seed = Union[int, Tensor]
+
+_NO_CONTEXT = nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (nothing to enter where it already is)."""
+    return _NO_CONTEXT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def require_gpu(device: torch.device, **tensors: Optional[Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise ValueError(f"{name} must be a tensor on {device if device.type == 'cuda' else 'the GPU'}")
+
+
+def row_stride(name: str, t: Tensor, cols: int) -> int:
+    """Distance of the rows of ``t`` (its last dimension) in elements: the elements of a row must lie
+    together and the rows at one common distance."""
+    if t.is_contiguous():
+        return cols
+    if t.dim() > 0 and (cols == 1 or t.stride(-1) == 1):
+        stride, extent = None, 1  # over the leading dimensions, the innermost first
+        for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if stride is None:
+                stride, extent = step, size
+            elif step == stride * extent:
+                extent *= size
+            else:
+                break
+        else:
+            return cols if stride is None else stride
+    raise ValueError(f"{name}: the elements of a row must lie together and its rows at one distance (shape {tuple(t.shape)}, "
+                     f"strides {tuple(t.stride())})")
+
+
+def with_even_rows(t: Tensor) -> Tensor:
+    """``t``, or a contiguous copy where its rows do not lie at one distance (gradients that arrive
+    from a broadcast or a transposition)."""
+    try:
+        row_stride("gradient", t, t.shape[-1] if t.dim() else 1)
+        return t
+    except ValueError:
+        return t.contiguous()
+
+
+def dropout_record(device: torch.device, p: float, seed: Seed, substream: int, first_index: int) -> "_C.Dropout":
+    if not 0 <= substream < 1 << 32:
+        raise ValueError("substream must be a 32-bit number")
+    if not 0 <= first_index < 1 << 62:
+        raise ValueError("first_index must be a number of 62 bits")
+    if isinstance(seed, Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ValueError("a seed in GPU memory is one int64 element")
+        require_gpu(device, seed=seed)
+        return _C.Dropout(p, 0, seed.data_ptr(), first_index, substream, 0)
+    if not 0 <= seed < 1 << 64:
+        raise ValueError("seed must be a 64-bit number")
+    return _C.Dropout(p, seed, None, first_index, substream, 0)
+
+
+def token_record(tokens: Tensor, first_row: int, padding: Optional[int]) -> Tuple["_C.Tokens", int]:
+    """The C record of ``tokens`` and how many they are."""
+    if tokens.dtype == torch.int64:
+        size = 8
+    elif tokens.dtype == torch.int32:
+        size = 4
+    else:
+        raise ValueError(f"tokens must be int64 or int32, not {tokens.dtype}")
+    if not 0 <= first_row < 1 << 62:
+        raise ValueError("first_row must not be negative")
+    n = tokens.numel()
+    if tokens.is_contiguous():
+        outer, inner, outer_stride, inner_stride = 1, n, 0, 1
+    elif tokens.dim() == 1:
+        outer, inner, outer_stride, inner_stride = 1, n, 0, tokens.stride(0)
+    elif tokens.dim() == 2:
+        (outer, inner), (outer_stride, inner_stride) = tokens.shape, tokens.stride()
+    else:
+        raise ValueError("tokens of more than two dimensions must be contiguous")
+    if padding is None:
+        padding = _C.NO_PADDING
+    elif not -(1 << 63) < padding < 1 << 63:
+        raise ValueError("padding_token must be a 64-bit number")
+    return _C.Tokens(tokens.data_ptr(), outer, inner, outer_stride, inner_stride, first_row, padding, size, 0), n

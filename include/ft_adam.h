@@ -339,6 +339,73 @@ int ft_synth_fill(void* out, int dtype, size_t n, uint64_t seed, uint32_t substr
 int ft_synth_fill_host(void* out, int dtype, size_t n, uint64_t seed, uint32_t substream, uint64_t first_index,
                        int kind, float scale);
 
+/* ---- rows of an embedding table ----------------------------------------------------------------
+ * The embedding is the largest of the parameters that belong to no layer unit
+ * (flextrain/optimizer.py:155-215). The reference leaves its lookup and its gradient to torch: a dense
+ * gradient of the whole table per micro-batch, added element by element to the gradient accumulator
+ * (:194-215). Here the lookup reads the low-precision copy that the update writes, and the gradient
+ * goes row by row straight into the accumulator: only rows that a token names are touched.
+ *
+ * ft_tokens_t: outer x inner token ids (id_bytes 4 or 8, signed; element strides), token i at outer
+ * index i / inner. Id t is row t - first_row of the table; an id outside first_row ... first_row +
+ * rows - 1 (another shard of the vocabulary) is no error: its row reads as zero and has no gradient.
+ * padding: an id without a gradient (its row is looked up like any other), FT_NO_PADDING for none.
+ *
+ * ft_dropout_t: element i of a call (row-major over its rows) is dropped with probability p by the
+ * counter generator under (seed, substream, first_index + i); the others are multiplied with
+ * 1 / (1 - p). The mask is never stored: a call with the same values makes it again. p is honoured to
+ * 2^-48. seed_dev: NULL, or 8 bytes of device memory holding the seed (it replaces `seed`), for a
+ * recorded pass whose masks are to differ between replays. The mask and ft_synth_fill share the
+ * generator: use other substreams for them.
+ *
+ * Strides are in elements; rows may lie apart, the elements of a row lie together. Pointers need the
+ * alignment of their element type. Tables have at most 2^31 - 1 rows of at most 2^24 elements, calls at
+ * most 2^31 - 1 tokens. No call allocates or waits, all may be recorded into a HIP graph.
+ *
+ * ft_embedding_lookup: out[i][c] = scale * table[row(i)][c], with drop != NULL then dropped out; one
+ * product in fp32 per element (by scale / (1 - p), rounded once), rounded to out's type. */
+#define FT_NO_PADDING INT64_MIN
+typedef struct ft_tokens_t {
+    const void* ids;
+    size_t outer, inner;
+    size_t outer_stride, inner_stride;
+    int64_t first_row;
+    int64_t padding;
+    int32_t id_bytes;
+    int32_t reserved; /* 0 */
+} ft_tokens_t;
+typedef struct ft_dropout_t {
+    double p; /* 0 ... 1 */
+    uint64_t seed;
+    const void* seed_dev;
+    uint64_t first_index;
+    uint32_t substream;
+    uint32_t reserved; /* 0 */
+} ft_dropout_t;
+int ft_embedding_lookup(const ft_tokens_t* tokens, const void* table, int table_dtype, size_t rows, size_t table_stride, void* out,
+                        int out_dtype, size_t out_stride, size_t cols, double scale, const ft_dropout_t* drop, void* stream);
+
+/* ft_embedding_grad: the lookup's gradient. g holds one row per token; acc[v][c] += scale * the sum of
+ * g[i][c] over the tokens i of row v that are no padding (accumulate != 0; other rows are not touched),
+ * or acc = that sum with zeros in the rows without a token (accumulate == 0). drop: the lookup's. Sums
+ * are kept in fp32 and rounded to acc's type once. Tokens are sorted and added in an order that
+ * depends on the arguments alone: the same call gives the same bits.
+ * workspace: ft_embedding_grad_workspace_bytes(outer * inner, rows, cols) bytes of device memory,
+ * 16-byte aligned, which calls that may overlap in time must not share (0 for few tokens: NULL will do). */
+size_t ft_embedding_grad_workspace_bytes(size_t n_tokens, size_t rows, size_t cols);
+int ft_embedding_grad(const ft_tokens_t* tokens, const void* g, int g_dtype, size_t g_stride, void* acc, int acc_dtype, size_t rows,
+                      size_t acc_stride, size_t cols, double scale, int accumulate, const ft_dropout_t* drop, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ---- dropout -----------------------------------------------------------------------------------
+ * out = [residual +] dropout(x) for rows x cols elements (see ft_dropout_t above). residual (NULL: none)
+ * has out's type; out may be x or residual itself where type and strides agree. A dropped element
+ * contributes 0, whatever x holds there. The gradient of x is the same call on the gradient of out,
+ * without residual; that of residual is the gradient of out. No counterpart in the reference, whose
+ * models drop out through torch with a stored mask. */
+int ft_dropout(const void* x, int x_dtype, size_t x_stride, const void* residual, size_t residual_stride, void* out, int out_dtype,
+               size_t out_stride, size_t rows, size_t cols, const ft_dropout_t* drop, void* stream);
+
 /* ---- launch tuning ------------------------------------------------------------------------
  * adam_waves_per_cu: how many 64-lane workgroups of the update kernel (16-bit gradients: 56 bytes
  * of loads in flight per lane) may be resident on one compute unit; kernels with fewer bytes per
