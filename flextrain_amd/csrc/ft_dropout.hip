@@ -30,40 +30,53 @@ struct DropoutPass {
     ftc::DropoutArgs drop;
 };
 
-// One unit of eight elements per lane. FLAT: the arrays are contiguous and count as one row.
+// One unit per lane. FLAT: the arrays are contiguous and count as one row.
 template <int XT, int OT, bool RES, bool DROP, bool FLAT>
 __global__ __launch_bounds__(kBlock) void dropout_kernel(DropoutPass a)
 {
-    const uint64_t t = static_cast<uint64_t>(blockIdx.x) * kBlock + threadIdx.x;
-    if (t >= a.units) return;
-    uint64_t row, col;
+    constexpr int U = row_unit<XT, OT>();
+    uint64_t xi, ri, oi, base;  // elements of the arrays; mask index of the unit: base + offset
+    uint32_t offset, count = U;
     if constexpr (FLAT) {
-        row = 0;
-        col = (a.first_unit + t) * kRowUnit;
+        base = (a.first_unit + static_cast<uint64_t>(blockIdx.x) * kBlock) * U;  // wave-uniform
+        offset = threadIdx.x * U;
+        if (a.cols - base < kBlock * U) {  // the last workgroup
+            const uint32_t left = static_cast<uint32_t>(a.cols - base);
+            if (offset >= left) return;
+            if (left - offset < U) count = left - offset;
+        }
+        xi = ri = oi = base + offset;
     } else {
-        const uint32_t r = static_cast<uint32_t>(t) / a.units_per_row;
-        row = a.first_row + r;
-        col = static_cast<uint64_t>(static_cast<uint32_t>(t) - r * a.units_per_row) * kRowUnit;
+        const uint32_t t = blockIdx.x * kBlock + threadIdx.x;
+        if (t >= a.units) return;
+        const uint32_t r = t / a.units_per_row;
+        const uint64_t row = a.first_row + r;
+        offset = (t - r * a.units_per_row) * U;
+        if (a.cols - offset < U) count = static_cast<uint32_t>(a.cols) - offset;
+        xi = row * a.x_stride + offset;
+        ri = row * a.residual_stride + offset;
+        oi = row * a.out_stride + offset;
+        base = row * a.cols;
     }
-    const uint64_t left = a.cols - col;
-    const uint32_t count = left < kRowUnit ? static_cast<uint32_t>(left) : kRowUnit;
-    const uint64_t xi = row * a.x_stride + col, oi = row * a.out_stride + col;
-    RowBits<XT> xb;
-    RowBits<OT> rb;
-    if (count == kRowUnit) {
-        xb = row_load8<XT, true>(a.x, xi);
-        if constexpr (RES) rb = row_load8<OT, true>(a.residual, row * a.residual_stride + col);
+    RowBits<XT, U> xb;
+    RowBits<OT, U> rb;
+    if (count == U) {
+        xb = row_load<XT, U, true>(a.x, xi);
+        if constexpr (RES) rb = row_load<OT, U, true>(a.residual, ri);
     } else {
-        xb = row_load_some<XT>(a.x, xi, count);
-        if constexpr (RES) rb = row_load_some<OT>(a.residual, row * a.residual_stride + col, count);
+        xb = row_load_some<XT, U>(a.x, xi, count);
+        if constexpr (RES) rb = row_load_some<OT, U>(a.residual, ri, count);
     }
-    bool keep[kRowUnit];
-    if constexpr (DROP) ftc::keep8(keep, ftc::dropout_key(a.drop), a.drop.first + row * a.cols + col, a.drop.hi, a.drop.lo);
-    float x[kRowUnit], y[kRowUnit];
-    row_floats<XT>(x, xb);
-    if constexpr (RES) row_floats<OT>(y, rb);
+    bool keep[U];
+    if constexpr (DROP) {
+        const uint64_t b = a.drop.first + base;
+        ftc::keep_units<U>(keep, ftc::group_argument(ftc::dropout_key(a.drop), b, offset), static_cast<uint32_t>(b) & 3u, a.drop);
+    }
+    float x[U], y[U];
+    row_floats<XT, U>(x, xb);
+    if constexpr (RES) row_floats<OT, U>(y, rb);
 #pragma unroll
-    for (int k = 0; k < kRowUnit; ++k) {
+    for (int k = 0; k < U; ++k) {
         if constexpr (DROP) {  // a dropped element is 0 whatever x holds
             if constexpr (RES)
                 y[k] = keep[k] ? __builtin_fmaf(x[k], a.drop.factor, y[k]) : y[k];
@@ -76,19 +89,20 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(DropoutPass a)
                 y[k] = x[k];
         }
     }
-    if (count == kRowUnit)
-        row_store8<OT, true>(a.out, oi, y);
+    if (count == U)
+        row_store<OT, U, true>(a.out, oi, y);
     else
-        row_store_some<OT>(a.out, oi, y, count);
+        row_store_some<OT, U>(a.out, oi, y, count);
 }
 
 template <int XT, int OT, bool RES, bool DROP>
 int launch(DropoutPass a, uint64_t rows, hipStream_t stream)
 {
+    constexpr int U = row_unit<XT, OT>();
     const bool flat = rows == 1 || (a.x_stride == a.cols && a.out_stride == a.cols && (!RES || a.residual_stride == a.cols));
     if (flat) {
         a.cols *= rows;
-        const uint64_t units = (a.cols + kRowUnit - 1) / kRowUnit;
+        const uint64_t units = (a.cols + U - 1) / U;
         constexpr uint64_t kPiece = 1ull << 31;  // lanes per launch
         for (a.first_unit = 0; a.first_unit < units; a.first_unit += kPiece) {
             a.units = units - a.first_unit < kPiece ? units - a.first_unit : kPiece;
@@ -98,7 +112,7 @@ int launch(DropoutPass a, uint64_t rows, hipStream_t stream)
         }
         return FT_OK;
     }
-    a.units_per_row = static_cast<uint32_t>((a.cols + kRowUnit - 1) / kRowUnit);
+    a.units_per_row = static_cast<uint32_t>((a.cols + U - 1) / U);
     const uint64_t piece = (1ull << 31) / a.units_per_row;  // rows per launch; cols is below 2^31
     for (a.first_row = 0; a.first_row < rows; a.first_row += piece) {
         const uint64_t now = rows - a.first_row < piece ? rows - a.first_row : piece;

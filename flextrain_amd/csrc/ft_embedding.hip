@@ -44,11 +44,43 @@ struct Tokens {
             const uint32_t o = i / inner;
             at = o * outer_stride + (i - o * inner) * inner_stride;
         }
-        const int64_t id = wide ? static_cast<const int64_t*>(ids)[at] : static_cast<int64_t>(static_cast<const int32_t*>(ids)[at]);
+        return row_of(wide ? static_cast<const int64_t*>(ids)[at] : static_cast<int64_t>(static_cast<const int32_t*>(ids)[at]));
+    }
+
+    __device__ __forceinline__ uint32_t row_of(int64_t id) const
+    {
         const uint64_t r = static_cast<uint64_t>(id) - first_row;
         return r < rows && id != padding ? static_cast<uint32_t>(r) : kNoRow;
     }
 };
+
+// The rows of the tokens base + 64 r (base: a lane's first token), kNoRow behind the last. All ids are
+// fetched before the first is looked at: one wait for all of them.
+template <int ITEMS>
+__device__ __forceinline__ void load_rows(uint32_t (&key)[ITEMS], const Tokens& t, uint32_t base)
+{
+    auto fetch = [&](auto element) {
+        using T = decltype(element);
+        T id[ITEMS];
+        const T* ids = static_cast<const T*>(t.ids);
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) {
+            const uint32_t i = base + r * kLanes;
+            id[r] = ids[i < t.n ? i : t.n - 1];
+        }
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) key[r] = base + r * kLanes < t.n ? t.row_of(id[r]) : kNoRow;
+    };
+    if (t.inner == t.n && t.inner_stride == 1) {
+        if (t.wide)
+            fetch(int64_t{});
+        else
+            fetch(int32_t{});
+    } else {
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) key[r] = base + r * kLanes < t.n ? t.row(base + r * kLanes) : kNoRow;
+    }
+}
 
 // ---- lookup -----------------------------------------------------------------------------------
 struct LookupPass {
@@ -67,54 +99,59 @@ struct LookupPass {
 template <int TT, int OT, bool DROP, int LPR, int K>
 __global__ __launch_bounds__(256) void embedding_lookup_kernel(LookupPass a)
 {
+    constexpr int U = row_unit<TT, OT>();
     const uint32_t wave = blockIdx.x * 4u + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
     uint32_t token, col;
     if constexpr (LPR == kLanes) {
         const uint32_t w = __builtin_amdgcn_readfirstlane(wave);
         token = w / a.chunks;
-        col = ((w - token * a.chunks) * K * kLanes + lane) * kRowUnit;
+        col = ((w - token * a.chunks) * K * kLanes + lane) * U;
     } else {
         token = wave * (kLanes / LPR) + lane / LPR;
-        col = (lane % LPR) * kRowUnit;
+        col = (lane % LPR) * U;
     }
     if (token >= a.tokens.n) return;
     const uint32_t row = a.tokens.row(token);
     const uint64_t from = static_cast<uint64_t>(row) * a.table_stride, to = token * a.out_stride;
-    RowBits<TT> bits[K];
+    RowBits<TT, U> bits[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const uint32_t c = col + k * kLanes * kRowUnit;
+        const uint32_t c = col + k * kLanes * U;
         if (row == kNoRow || c >= a.cols) continue;
-        bits[k] = a.cols - c >= kRowUnit ? row_load8<TT, false>(a.table, from + c) : row_load_some<TT>(a.table, from + c, a.cols - c);
+        bits[k] = a.cols - c >= U ? row_load<TT, U, false>(a.table, from + c) : row_load_some<TT, U>(a.table, from + c, a.cols - c);
     }
     uint64_t key = 0;
     if constexpr (DROP) key = ftc::dropout_key(a.drop);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const uint32_t c = col + k * kLanes * kRowUnit;
+        const uint32_t c = col + k * kLanes * U;
         if (c >= a.cols) continue;
-        float x[kRowUnit] = {};
+        float x[U] = {};
         if (row != kNoRow) {
-            row_floats<TT>(x, bits[k]);
-            bool keep[kRowUnit];
-            if constexpr (DROP) ftc::keep8(keep, key, a.drop.first + static_cast<uint64_t>(token) * a.cols + c, a.drop.hi, a.drop.lo);
+            row_floats<TT, U>(x, bits[k]);
+            bool keep[U];
+            if constexpr (DROP) {
+                const uint64_t b = a.drop.first + static_cast<uint64_t>(token) * a.cols;
+                ftc::keep_units<U>(keep, ftc::group_argument(key, b, c), static_cast<uint32_t>(b) & 3u, a.drop);
+            }
 #pragma unroll
-            for (int j = 0; j < kRowUnit; ++j) {
+            for (int j = 0; j < U; ++j) {
                 x[j] *= a.factor;
                 if constexpr (DROP) x[j] = keep[j] ? x[j] : 0.0f;
             }
         }
-        if (a.cols - c >= kRowUnit)
-            row_store8<OT, true>(a.out, to + c, x);
+        if (a.cols - c >= U)
+            row_store<OT, U, true>(a.out, to + c, x);
         else
-            row_store_some<OT>(a.out, to + c, x, a.cols - c);
+            row_store_some<OT, U>(a.out, to + c, x, a.cols - c);
     }
 }
 
 template <int TT, int OT, bool DROP>
 int launch_lookup(LookupPass a, hipStream_t stream)
 {
-    const uint32_t units = (a.cols + kRowUnit - 1) / kRowUnit;
+    constexpr int U = row_unit<TT, OT>();
+    const uint32_t units = (a.cols + U - 1) / U;
     auto go = [&](auto lpr, auto k) -> int {
         constexpr int LPR = decltype(lpr)::value, K = decltype(k)::value;
         a.chunks = (units + kLanes * K - 1) / (kLanes * K);
@@ -128,8 +165,11 @@ int launch_lookup(LookupPass a, hipStream_t stream)
     };
     using std::integral_constant;
     if (units <= 16) return go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-    if (static_cast<uint64_t>(a.tokens.n) * ((units + kLanes - 1) / kLanes) < 16384) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    return go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    // 16,376 rows of 4096 bf16 elements, one / two / four units per lane: 29 / 32 / 32 us; with dropout 45 / 33 / 33 us;
+    // 32,768 rows of 8192 fp16 elements into fp32: 268 / 202 / 226 us. Few rows need every wavefront they can get.
+    const bool few = static_cast<uint64_t>(a.tokens.n) * ((units + kLanes - 1) / kLanes) < 16384;
+    if (few || (U == 8 && !DROP)) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
 }
 
 // ---- gradient ---------------------------------------------------------------------------------
@@ -143,53 +183,67 @@ struct GradPass {
     float factor;
     ftc::DropoutArgs drop;
     // sorted tokens (long calls)
-    const uint32_t* row_s;
+    const uint32_t* row_s;   // tokens outside the table last, as row tokens.rows
     const uint32_t* pos_s;
     float* head;             // [groups][padded cols]: the end of a run that began in an earlier workgroup
     float* tail;             // the beginning of a run that goes on in the next one
+    uint32_t rotate;         // the rows' order is that of their numbers rotated right by this many bits
     uint32_t per_wave;       // sorted tokens per wavefront
     uint32_t groups;         // workgroups per block of columns
     uint32_t padded;         // columns rounded up to whole blocks
 };
 
-// The gradient's unit of eight elements of token `pos` at column `col`, masked.
-template <int GT, bool DROP>
-__device__ __forceinline__ void add_unit(float (&sum)[kRowUnit], const RowBits<GT>& bits, const GradPass& a, uint64_t key, uint32_t pos, uint32_t col)
+template <int DT, int U, bool NT>
+__device__ __forceinline__ RowBits<DT, U> load_unit(const void* base, uint64_t at, uint32_t count)
 {
-    float x[kRowUnit];
-    row_floats<GT>(x, bits);
+    return count == U ? row_load<DT, U, NT>(base, at) : row_load_some<DT, U>(base, at, count);
+}
+
+// Adds the gradient's unit of token `pos` at column `col`, masked.
+template <int GT, int U, bool DROP>
+__device__ __forceinline__ void add_unit(float (&sum)[U], const RowBits<GT, U>& bits, const GradPass& a, uint64_t key, uint32_t pos, uint32_t col)
+{
+    float x[U];
+    row_floats<GT, U>(x, bits);
     if constexpr (DROP) {
-        bool keep[kRowUnit];
-        ftc::keep8(keep, key, a.drop.first + static_cast<uint64_t>(pos) * a.cols + col, a.drop.hi, a.drop.lo);
+        bool keep[U];
+        const uint64_t b = a.drop.first + static_cast<uint64_t>(pos) * a.cols;
+        ftc::keep_units<U>(keep, ftc::group_argument(key, b, col), static_cast<uint32_t>(b) & 3u, a.drop);
 #pragma unroll
-        for (int j = 0; j < kRowUnit; ++j) sum[j] += keep[j] ? x[j] : 0.0f;
+        for (int j = 0; j < U; ++j) sum[j] += keep[j] ? x[j] : 0.0f;
     } else {
 #pragma unroll
-        for (int j = 0; j < kRowUnit; ++j) sum[j] += x[j];
+        for (int j = 0; j < U; ++j) sum[j] += x[j];
     }
 }
 
-template <int GT>
-__device__ __forceinline__ RowBits<GT> load_unit(const GradPass& a, uint32_t pos, uint32_t col, uint32_t count)
-{
-    const uint64_t at = static_cast<uint64_t>(pos) * a.g_stride + col;
-    if (count == kRowUnit) return row_load8<GT, true>(a.g, at);
-    return row_load_some<GT>(a.g, at, count);
-}
-
-// acc[row] (+)= factor * sum: the one rounding to the accumulator's type.
-template <int AT>
-__device__ __forceinline__ void finish_unit(const GradPass& a, uint32_t row, uint32_t col, uint32_t count, float (&sum)[kRowUnit])
+// acc[row] = [old +] factor * sum: the one rounding to the accumulator's type.
+template <int AT, int U>
+__device__ __forceinline__ void finish_unit(const GradPass& a, uint32_t row, uint32_t col, uint32_t count, const float (&sum)[U],
+                                            const RowBits<AT, U>& old)
 {
     const uint64_t at = static_cast<uint64_t>(row) * a.acc_stride + col;
-    float x[kRowUnit] = {};
-    if (a.accumulate) row_floats<AT>(x, count == kRowUnit ? row_load8<AT, false>(a.acc, at) : row_load_some<AT>(a.acc, at, count));
+    float x[U];
+    if (a.accumulate) {
+        row_floats<AT, U>(x, old);
 #pragma unroll
-    for (int j = 0; j < kRowUnit; ++j) x[j] = a.accumulate ? __builtin_fmaf(sum[j], a.factor, x[j]) : sum[j] * a.factor;
-    if (count == kRowUnit)
-        row_store8<AT, false>(a.acc, at, x);
+        for (int j = 0; j < U; ++j) x[j] = __builtin_fmaf(sum[j], a.factor, x[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j) x[j] = sum[j] * a.factor;
+    }
+    if (count == U)
+        row_store<AT, U, true>(a.acc, at, x);
     else
-        row_store_some<AT>(a.acc, at, x, count);
+        row_store_some<AT, U>(a.acc, at, x, count);
+}
+
+template <int AT, int U>
+__device__ __forceinline__ RowBits<AT, U> load_old(const GradPass& a, uint32_t row, uint32_t col, uint32_t count)
+{
+    RowBits<AT, U> old{};
+    if (a.accumulate) old = load_unit<AT, U, false>(a.acc, static_cast<uint64_t>(row) * a.acc_stride + col, count);
+    return old;
 }
 
 // Short calls: one launch without sorting. The wavefront of a token looks through all tokens (two
@@ -199,6 +253,7 @@ constexpr uint32_t kShortTokens = 2 * kLanes;
 template <int GT, int AT, bool DROP>
 __global__ __launch_bounds__(kLanes) void embedding_grad_short_kernel(GradPass a)
 {
+    constexpr int U = row_unit<GT, AT>();
     const uint32_t lane = threadIdx.x, n = a.tokens.n, me = blockIdx.x;
     const uint32_t r0 = lane < n ? a.tokens.row(lane) : kNoRow;
     const uint32_t r1 = lane + kLanes < n ? a.tokens.row(lane + kLanes) : kNoRow;
@@ -207,15 +262,16 @@ __global__ __launch_bounds__(kLanes) void embedding_grad_short_kernel(GradPass a
     uint64_t m0 = __builtin_amdgcn_ballot_w64(r0 == mine), m1 = __builtin_amdgcn_ballot_w64(r1 == mine);
     const uint32_t first = m0 ? __builtin_ctzll(m0) : kLanes + __builtin_ctzll(m1);
     if (first != me) return;
-    const uint32_t col = (blockIdx.y * kLanes + lane) * kRowUnit;
+    const uint32_t col = (blockIdx.y * kLanes + lane) * U;
     if (col >= a.cols) return;
-    const uint32_t count = a.cols - col < kRowUnit ? a.cols - col : kRowUnit;
+    const uint32_t count = a.cols - col < U ? a.cols - col : U;
+    const RowBits<AT, U> old = load_old<AT, U>(a, mine, col, count);
     uint64_t key = 0;
     if constexpr (DROP) key = ftc::dropout_key(a.drop);
-    float sum[kRowUnit] = {};
+    float sum[U] = {};
     while (m0 | m1) {
         uint32_t pos[4];
-        RowBits<GT> bits[4];
+        RowBits<GT, U> bits[4];
         int have = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -223,28 +279,40 @@ __global__ __launch_bounds__(kLanes) void embedding_grad_short_kernel(GradPass a
             pos[j] = m0 ? __builtin_ctzll(m0) : kLanes + __builtin_ctzll(m1);
             if (m0) m0 &= m0 - 1;
             else m1 &= m1 - 1;
-            bits[j] = load_unit<GT>(a, pos[j], col, count);
+            bits[j] = load_unit<GT, U, true>(a.g, static_cast<uint64_t>(pos[j]) * a.g_stride + col, count);
             have = j + 1;
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j < have) add_unit<GT, DROP>(sum, bits[j], a, key, pos[j], col);
+            if (j < have) add_unit<GT, U, DROP>(sum, bits[j], a, key, pos[j], col);
     }
-    finish_unit<AT>(a, mine, col, count, sum);
+    finish_unit<AT, U>(a, mine, col, count, sum, old);
 }
 
 // ---- sorting the tokens by row ------------------------------------------------------------------
-// Stable radix sort of (row, position), least significant digits first, tokens outside the table
-// behind all others (as row `rows`). A workgroup ranks a tile of 1024 * R tokens: wavefront w holds
-// 64 * R consecutive ones, 64 at a time, and counts them per digit in LDS counters of its own; lanes
-// with the same digit find each other with one ballot per bit of the digit, so ranks follow the order
-// of the tokens and no LDS atomic is needed. Calls of at most one tile sort in one launch, all
-// passes in LDS; longer ones take two launches a pass (count, place).
+// Stable: tokens of one row keep their order, so that sums do not depend on how workgroups run. Which
+// order the rows have among each other does not matter, as long as the clearing kernel knows it.
+//
+// Up to 16,384 tokens: one launch, no workgroup waits for another. Workgroup b looks through ALL
+// tokens (sixteen per thread at most), keeps those whose row ends in the byte b, counts those that go
+// in front of them, and sorts its own by the row's other bits in LDS. That is 256 times the reading, all of it
+// from the L2, and takes 6 us where sorting in one workgroup took 23 us (8,192 tokens) and two passes of
+// two launches each 50 us (16,384).
+// More: radix sort by digits of at most nine bits, two launches a pass (count, place).
+//
+// Ranking inside a workgroup: wavefront w holds 64 * R consecutive items, 64 at a time, and counts them
+// per digit in LDS counters of its own; lanes with the same digit find each other with one ballot per bit
+// of the digit, so ranks follow the items' order and no LDS atomic is needed.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kLanes;
-constexpr int kSortItems = 8;                             // R at most
-constexpr uint32_t kSortTile = kSortThreads * kSortItems;
 constexpr uint32_t kMaxDigitBits = 9;
+constexpr uint32_t kBucketBits = 8;
+constexpr uint32_t kBuckets = 1u << kBucketBits;
+constexpr uint32_t kBucketPosBits = 14;
+constexpr uint32_t kBucketTokens = 1u << kBucketPosBits;       // tokens of a one-launch sort
+constexpr uint64_t kBucketRows = 1ull << (32 - kBucketPosBits + kBucketBits);  // its rows: the other bits share 32 with the position
+constexpr uint32_t kPairTokens = 512;                          // up to here a bucket is sorted by comparing all pairs
+constexpr uint32_t kDirectTiles = 64;                          // up to here every tile adds up the others' counts itself
 
 struct SortPass {
     Tokens tokens;
@@ -252,21 +320,31 @@ struct SortPass {
     const uint32_t* pos_in;
     uint32_t* row_out;
     uint32_t* pos_out;
-    uint32_t* count;         // [tiles][1 << digit_bits]
+    uint32_t* count;         // [tiles + 1][1 << digit_bits]; the last row: all tiles together (scanned counts only)
     uint32_t shift, digit_bits, passes, tiles;
+    int32_t scanned;         // count[t] holds the sum over the tiles before t
 };
 
-__device__ __forceinline__ uint32_t sort_key(const Tokens& t, uint32_t i)
+// The radix sort's items base + 64 r: rows (of tokens outside the table: `rows`) and positions.
+template <int ITEMS>
+__device__ __forceinline__ void load_items(uint32_t (&key)[ITEMS], const SortPass& a, uint32_t base)
 {
-    const uint32_t r = t.row(i);
-    return r == kNoRow ? t.rows : r;
+    if (a.row_in) {
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) key[r] = a.row_in[base + r * kLanes < a.tokens.n ? base + r * kLanes : a.tokens.n - 1];
+    } else {
+        load_rows<ITEMS>(key, a.tokens, base);
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) key[r] = key[r] == kNoRow ? a.tokens.rows : key[r];
+    }
 }
 
 // Lanes of the wavefront whose digit is this lane's; `active` lanes only.
-__device__ __forceinline__ uint64_t same_digit(uint32_t digit, uint32_t bits, bool active)
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool active)
 {
     uint64_t m = __builtin_amdgcn_ballot_w64(active);
-    for (uint32_t b = 0; b < bits; ++b) {
+#pragma unroll
+    for (uint32_t b = 0; b < kMaxDigitBits; ++b) {
         const bool one = digit >> b & 1u;
         const uint64_t v = __builtin_amdgcn_ballot_w64(one);
         m &= one ? v : ~v;
@@ -274,8 +352,8 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, uint32_t bits, bo
     return m;
 }
 
-// Sum over the threads before this one (1024 threads); total of all in *total.
-__device__ __forceinline__ uint32_t exclusive_scan(uint32_t x, uint32_t* wave_sums, uint32_t* total)
+// Sum over the threads before this one (1024 threads).
+__device__ __forceinline__ uint32_t exclusive_scan(uint32_t x, uint32_t* wave_sums)
 {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     uint32_t s = x;
@@ -287,20 +365,17 @@ __device__ __forceinline__ uint32_t exclusive_scan(uint32_t x, uint32_t* wave_su
     __syncthreads();
     if (lane == 63) wave_sums[wave] = s;
     __syncthreads();
-    uint32_t before = 0, all = 0;
+    uint32_t before = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kSortWaves; ++w) {
-        const uint32_t v = wave_sums[w];
-        before += w < wave ? v : 0;
-        all += v;
-    }
-    *total = all;
+    for (uint32_t w = 0; w < kSortWaves; ++w) before += w < wave ? wave_sums[w] : 0;
     return before + s - x;
 }
 
-// Ranks the tile's items by digit. counters[w][digit] ends as the number of the wavefront's items
-// with that digit; rank[] as the number of them in front of each item.
-__device__ __forceinline__ void rank_items(uint32_t (&rank)[kSortItems], const uint32_t (&key)[kSortItems], uint32_t r_count, uint32_t base, uint32_t n,
+// Ranks a tile's items by digit. Item r of lane l of wavefront w is item base + 64 r + l, base = 64 w r_count
+// from the tile's begin; those from n on do not exist. counters[w][digit] ends as the number of the wavefront's
+// items with that digit; rank[] as the number of them in front of each item.
+template <int ITEMS>
+__device__ __forceinline__ void rank_items(uint32_t (&rank)[ITEMS], const uint32_t (&key)[ITEMS], uint32_t r_count, uint32_t base, uint32_t n,
                                            uint32_t shift, uint32_t bits, uint32_t* counters)
 {
     const uint32_t lane = threadIdx.x & 63u, bins = 1u << bits;
@@ -308,179 +383,340 @@ __device__ __forceinline__ void rank_items(uint32_t (&rank)[kSortItems], const u
     for (uint32_t b = lane; b < bins; b += kLanes) mine[b] = 0;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-        if (static_cast<uint32_t>(r) >= r_count) break;
-        const bool active = base + r * kLanes + lane < n;
-        const uint32_t digit = key[r] >> shift & (bins - 1);
-        const uint64_t same = same_digit(digit, bits, active);
-        const uint32_t in_front = __builtin_popcountll(same & ((1ull << lane) - 1));
-        const uint32_t before = active ? mine[digit] : 0;
-        rank[r] = before + in_front;
-        __builtin_amdgcn_wave_barrier();
-        if (active && in_front == 0) mine[digit] = before + __builtin_popcountll(same);
-        __builtin_amdgcn_wave_barrier();
+    for (int r = 0; r < ITEMS; ++r) {
+        if (static_cast<uint32_t>(r) < r_count) {  // wave-uniform
+            const bool active = base + r * kLanes + lane < n;
+            const uint32_t digit = key[r] >> shift & (bins - 1);
+            const uint64_t same = same_digit(digit, active);
+            const uint32_t in_front = __builtin_popcountll(same & ((1ull << lane) - 1));
+            const uint32_t before = active ? mine[digit] : 0;
+            rank[r] = before + in_front;
+            __builtin_amdgcn_wave_barrier();
+            if (active && in_front == 0) mine[digit] = before + __builtin_popcountll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
 
-// One launch: at most kSortTile tokens.
-__global__ __launch_bounds__(kSortThreads) void sort_tile_kernel(SortPass a)
+// Turns the counters of rank_items into where each wavefront's items with a digit begin.
+__device__ __forceinline__ void scan_counters(uint32_t* counters, uint32_t bins, uint32_t* wave_sums)
 {
-    extern __shared__ uint32_t lds[];
-    const uint32_t bins = 1u << a.digit_bits, n = a.tokens.n;
-    uint32_t* counters = lds;                          // [kSortWaves][bins]
-    uint32_t* wave_sums = counters + kSortWaves * bins;  // [kSortWaves]
-    uint32_t* rows = wave_sums + kSortWaves;            // [r_count * 1024]
-    const uint32_t r_count = (n + kSortThreads - 1) / kSortThreads;
-    uint32_t* positions = rows + r_count * kSortThreads;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t base = wave * kLanes * r_count;
-    uint32_t key[kSortItems], pos[kSortItems], rank[kSortItems];
+    const uint32_t each = bins * kSortWaves / kSortThreads;  // counters per thread, 1 ... 8, in the order (digit, wavefront)
+    uint32_t local[8], sum = 0;
 #pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-        if (static_cast<uint32_t>(r) >= r_count) break;
-        pos[r] = base + r * kLanes + lane;
-        key[r] = pos[r] < n ? sort_key(a.tokens, pos[r]) : 0;
+    for (uint32_t k = 0; k < 8; ++k) {
+        const uint32_t e = threadIdx.x * each + k;
+        local[k] = k < each ? counters[(e % kSortWaves) * bins + e / kSortWaves] : 0;
+        sum += local[k];
     }
-    const uint32_t each = bins * kSortWaves / kSortThreads;  // counters a thread scans: 1 ... 8
-    for (uint32_t pass = 0; pass < a.passes; ++pass) {
-        const uint32_t shift = pass * a.digit_bits;
-        rank_items(rank, key, r_count, base, n, shift, a.digit_bits, counters);
+    uint32_t at = exclusive_scan(sum, wave_sums);
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) {
+        const uint32_t e = threadIdx.x * each + k;
+        if (k < each) counters[(e % kSortWaves) * bins + e / kSortWaves] = at;
+        at += local[k];
+    }
+}
+
+// ITEMS: tokens per thread, at least n / 1024.
+template <int ITEMS>
+__global__ __launch_bounds__(kSortThreads) void sort_buckets_kernel(SortPass a)
+{
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    __shared__ uint32_t kept[kSortWaves], in_front[kSortWaves], wave_sums[kSortWaves];
+    __shared__ __attribute__((aligned(16))) uint32_t pairs[kPairTokens + 4];
+    const uint32_t n = a.tokens.n, rows = a.tokens.rows, me = blockIdx.x;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr uint32_t per_wave = ITEMS * kLanes;
+    uint32_t* list = lds;  // the bucket's tokens (the row's other bits, then the position), each wavefront's from its own begin
+    uint32_t* counters = lds + ITEMS * kSortThreads;
+
+    uint32_t key[ITEMS];
+    load_rows<ITEMS>(key, a.tokens, wave * per_wave + lane);
+    uint32_t own = 0, before = 0;
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const bool valid = key[r] != kNoRow;
+        const uint32_t bucket = key[r] & (kBuckets - 1), i = wave * per_wave + r * kLanes + lane;
+        const uint64_t mine = __builtin_amdgcn_ballot_w64(valid && bucket == me);
+        before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(valid && bucket < me));
+        if (valid && bucket == me) list[wave * per_wave + own + __builtin_popcountll(mine & ((1ull << lane) - 1))] = key[r] >> kBucketBits << kBucketPosBits | i;
+        own += __builtin_popcountll(mine);
+    }
+    if (lane == 0) {
+        kept[wave] = own;
+        in_front[wave] = before;
+    }
+    __syncthreads();
+    uint32_t size = 0, begin = 0;  // of the bucket
+    uint32_t shares[kSortWaves];   // wavefronts' tokens
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWaves; ++w) {
+        shares[w] = __builtin_amdgcn_readfirstlane(kept[w]);
+        size += shares[w];
+        begin += __builtin_amdgcn_readfirstlane(in_front[w]);
+    }
+    if (me == kBuckets - 1)  // tokens outside the table, behind all others
+        for (uint32_t i = begin + size + threadIdx.x; i < n; i += kSortThreads) {
+            a.row_out[i] = rows;
+            a.pos_out[i] = 0;
+        }
+    if (size == 0) return;
+    auto in_order = [&](uint32_t i) {  // the bucket's token i, below size
+        uint32_t skipped = 0, at = i;
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWaves; ++w) {
+            at = i >= skipped ? w * per_wave + i - skipped : at;
+            skipped += shares[w];
+        }
+        return list[at];
+    };
+    auto write = [&](uint32_t to, uint32_t packed) {
+        a.row_out[begin + to] = packed >> kBucketPosBits << kBucketBits | me;
+        a.pos_out[begin + to] = packed & (kBucketTokens - 1);
+    };
+    if (size <= kPairTokens) {  // packed values are all different: the rank is the number of smaller ones
+        if (threadIdx.x < size + 4) pairs[threadIdx.x] = threadIdx.x < size ? in_order(threadIdx.x) : 0xffffffffu;
         __syncthreads();
-        // offsets in the order (digit, wavefront)
-        uint32_t local[8], sum = 0, total;
-#pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
-            if (k >= each) break;
-            const uint32_t e = threadIdx.x * each + k;
-            local[k] = counters[(e % kSortWaves) * bins + e / kSortWaves];
-            sum += local[k];
+        if (threadIdx.x >= size) return;
+        const uint32_t x = pairs[threadIdx.x];
+        uint32_t rank = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < size; j += 4) {
+            const u32x4 y = *reinterpret_cast<const u32x4*>(pairs + j);
+            rank += (y.x < x) + (y.y < x) + (y.z < x) + (y.w < x);
         }
-        uint32_t at = exclusive_scan(sum, wave_sums, &total);
+        write(rank, x);
+        return;
+    }
+    const uint32_t r_count = (size + kSortThreads - 1) / kSortThreads, first = wave * kLanes * r_count, bins = 1u << a.digit_bits;
+    uint32_t rank[ITEMS];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
-            if (k >= each) break;
-            const uint32_t e = threadIdx.x * each + k;
-            counters[(e % kSortWaves) * bins + e / kSortWaves] = at;
-            at += local[k];
-        }
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint32_t i = first + r * kLanes + lane;
+        key[r] = static_cast<uint32_t>(r) < r_count && i < size ? in_order(i) : 0;
+    }
+    for (uint32_t pass = 0; pass < a.passes; ++pass) {
+        const uint32_t shift = kBucketPosBits + pass * a.digit_bits;
+        rank_items<ITEMS>(rank, key, r_count, first, size, shift, a.digit_bits, counters);
+        __syncthreads();
+        scan_counters(counters, bins, wave_sums);
         __syncthreads();
         const bool last = pass + 1 == a.passes;
 #pragma unroll
-        for (int r = 0; r < kSortItems; ++r) {
-            if (static_cast<uint32_t>(r) >= r_count) break;
-            if (base + r * kLanes + lane >= n) continue;
-            const uint32_t to = counters[wave * bins + (key[r] >> shift & (bins - 1))] + rank[r];
-            if (last) {
-                a.row_out[to] = key[r];
-                a.pos_out[to] = pos[r];
-            } else {
-                rows[to] = key[r];
-                positions[to] = pos[r];
+        for (int r = 0; r < ITEMS; ++r) {
+            if (static_cast<uint32_t>(r) < r_count && first + r * kLanes + lane < size) {
+                const uint32_t to = counters[wave * bins + (key[r] >> shift & (bins - 1))] + rank[r];
+                if (last)
+                    write(to, key[r]);
+                else
+                    list[to] = key[r];
             }
         }
-        if (last) break;
+        if (last) return;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < kSortItems; ++r) {
-            if (static_cast<uint32_t>(r) >= r_count) break;
-            const uint32_t i = base + r * kLanes + lane;
-            if (i < n) {
-                key[r] = rows[i];
-                pos[r] = positions[i];
-            }
+        for (int r = 0; r < ITEMS; ++r) {
+            const uint32_t i = first + r * kLanes + lane;
+            if (static_cast<uint32_t>(r) < r_count && i < size) key[r] = list[i];
         }
         __syncthreads();
     }
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {  // no pass: all of one row
+        const uint32_t i = first + r * kLanes + lane;
+        if (static_cast<uint32_t>(r) < r_count && i < size) write(i, key[r]);
+    }
 }
 
-// Long calls, first launch of a pass: how often each digit occurs in each tile.
+// Radix sort, first launch of a pass: how often each digit occurs in each tile.
+template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortPass a)
 {
-    extern __shared__ uint32_t lds[];
-    const uint32_t bins = 1u << a.digit_bits, n = a.tokens.n;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t base = blockIdx.x * kSortTile + wave * kLanes * kSortItems;
-    uint32_t key[kSortItems], rank[kSortItems];
-#pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-        const uint32_t i = base + r * kLanes + lane;
-        key[r] = i < n ? (a.row_in ? a.row_in[i] : sort_key(a.tokens, i)) : 0;
-    }
-    rank_items(rank, key, kSortItems, base, n, a.shift, a.digit_bits, lds);
+    __shared__ uint32_t counters[1u << kMaxDigitBits];
+    const uint32_t bins = 1u << a.digit_bits;
+    const uint32_t base = (blockIdx.x * kSortWaves + (threadIdx.x >> 6)) * kLanes * ITEMS + (threadIdx.x & 63u);
+    uint32_t key[ITEMS];
+    load_items<ITEMS>(key, a, base);
+    if (threadIdx.x < bins) counters[threadIdx.x] = 0;
     __syncthreads();
-    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
-        uint32_t sum = 0;
-        for (uint32_t w = 0; w < kSortWaves; ++w) sum += lds[w * bins + b];
-        a.count[blockIdx.x * bins + b] = sum;
-    }
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+        if (base + r * kLanes < a.tokens.n) __hip_atomic_fetch_add(&counters[key[r] >> a.shift & (bins - 1)], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    __syncthreads();
+    if (threadIdx.x < bins) a.count[static_cast<uint64_t>(blockIdx.x) * bins + threadIdx.x] = counters[threadIdx.x];
 }
 
-// Second launch of a pass: every tile adds up where its digits begin and moves its tokens there.
+// Many tiles: turns their counts into sums over the tiles before. A workgroup has 64 digits, a
+// wavefront of it one sixteenth of the tiles.
+__global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(SortPass a)
+{
+    __shared__ uint32_t part[kSortWaves][kLanes];
+    const uint32_t bins = 1u << a.digit_bits, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t* count = a.count + blockIdx.x * kLanes + lane;
+    const uint32_t lo = static_cast<uint64_t>(a.tiles) * wave / kSortWaves, hi = static_cast<uint64_t>(a.tiles) * (wave + 1) / kSortWaves;
+    uint32_t sum = 0;
+#pragma unroll 8
+    for (uint32_t t = lo; t < hi; ++t) sum += count[static_cast<uint64_t>(t) * bins];
+    part[wave][lane] = sum;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (uint32_t w = 0; w < kSortWaves; ++w) {
+        before += w < wave ? part[w][lane] : 0;
+        all += part[w][lane];
+    }
+#pragma unroll 8
+    for (uint32_t t = lo; t < hi; ++t) {
+        const uint32_t c = count[static_cast<uint64_t>(t) * bins];
+        count[static_cast<uint64_t>(t) * bins] = before;
+        before += c;
+    }
+    if (wave == 0) count[static_cast<uint64_t>(a.tiles) * bins] = all;
+}
+
+// Last launch of a pass: every tile moves its tokens to where their digits begin.
+template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortPass a)
 {
-    extern __shared__ uint32_t lds[];
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    __shared__ uint32_t wave_sums[kSortWaves];
     const uint32_t bins = 1u << a.digit_bits, n = a.tokens.n;
-    uint32_t* counters = lds;                            // [kSortWaves][bins]
-    uint32_t* wave_sums = counters + kSortWaves * bins;    // [kSortWaves]
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t base = blockIdx.x * kSortTile + wave * kLanes * kSortItems;
-    uint32_t key[kSortItems], pos[kSortItems], rank[kSortItems];
+    const uint32_t base = (blockIdx.x * kSortWaves + wave) * kLanes * ITEMS;
+    uint32_t key[ITEMS], pos[ITEMS], rank[ITEMS];
+    load_items<ITEMS>(key, a, base + lane);
 #pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         const uint32_t i = base + r * kLanes + lane;
-        key[r] = i < n ? (a.row_in ? a.row_in[i] : sort_key(a.tokens, i)) : 0;
-        pos[r] = i < n ? (a.row_in ? a.pos_in[i] : i) : 0;
+        pos[r] = a.row_in && i < n ? a.pos_in[i] : i;
     }
-    rank_items(rank, key, kSortItems, base, n, a.shift, a.digit_bits, counters);
-    __syncthreads();
-    // this digit in the tiles before this one, and in all tiles
-    uint32_t before = 0, all = 0, total;
-    if (threadIdx.x < bins) {
-        for (uint32_t t = 0; t < a.tiles; ++t) {
-            const uint32_t c = a.count[t * bins + threadIdx.x];
+    // this digit in the tiles before this one, and in all tiles: two threads per digit add half of the tiles each
+    __shared__ uint32_t halves[2][1u << kMaxDigitBits];
+    uint32_t before = 0, all = 0;
+    if (a.scanned) {
+        if (threadIdx.x < bins) {
+            before = a.count[static_cast<uint64_t>(blockIdx.x) * bins + threadIdx.x];
+            all = a.count[static_cast<uint64_t>(a.tiles) * bins + threadIdx.x];
+        }
+    } else if (threadIdx.x < 2 * bins) {
+        const uint32_t half = threadIdx.x >= bins, digit = threadIdx.x - half * bins;
+#pragma unroll 16
+        for (uint32_t t = half; t < a.tiles; t += 2) {
+            const uint32_t c = a.count[t * bins + digit];
             before += t < blockIdx.x ? c : 0;
             all += c;
         }
+        if (half) {
+            halves[0][digit] = before;
+            halves[1][digit] = all;
+        }
     }
-    uint32_t at = exclusive_scan(all, wave_sums, &total) + before;
+    rank_items<ITEMS>(rank, key, ITEMS, base, n, a.shift, a.digit_bits, lds);
+    __syncthreads();
+    if (threadIdx.x < bins && !a.scanned) {
+        before += halves[0][threadIdx.x];
+        all += halves[1][threadIdx.x];
+    }
+    uint32_t at = exclusive_scan(threadIdx.x < bins ? all : 0, wave_sums) + before;
     if (threadIdx.x < bins) {
+        uint32_t c[kSortWaves];
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWaves; ++w) c[w] = lds[w * bins + threadIdx.x];
+#pragma unroll
         for (uint32_t w = 0; w < kSortWaves; ++w) {
-            const uint32_t c = counters[w * bins + threadIdx.x];
-            counters[w * bins + threadIdx.x] = at;
-            at += c;
+            lds[w * bins + threadIdx.x] = at;
+            at += c[w];
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         if (base + r * kLanes + lane >= n) continue;
-        const uint32_t to = counters[wave * bins + (key[r] >> a.shift & (bins - 1))] + rank[r];
+        const uint32_t to = lds[wave * bins + (key[r] >> a.shift & (bins - 1))] + rank[r];
         a.row_out[to] = key[r];
         a.pos_out[to] = pos[r];
     }
 }
 
+// ---- rows without a token ----------------------------------------------------------------------
+// A gradient that is written, not added: the other rows become zero. A workgroup owns 64 rows; each
+// lane looks its row up among the tokens (binary search in the sorted ones, all of them in a short
+// call).
+template <int AT>
+__device__ __forceinline__ void clear_rows(const GradPass& a, uint32_t block)
+{
+    constexpr int U = AT == FT_F32 ? 4 : 8;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n = a.tokens.n, first = block * kLanes, row = first + lane, waves = blockDim.x >> 6;
+    bool met = false;
+    if (a.row_s) {
+        auto order = [&](uint32_t r) { return r >= a.tokens.rows ? kNoRow : (r >> a.rotate) | (a.rotate ? r << (32 - a.rotate) : 0); };
+        const uint32_t mine = order(row);
+        uint32_t lo = 0, hi = n;  // the first sorted token of a row not in front of this one
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (order(a.row_s[mid]) < mine)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        met = lo < n && a.row_s[lo] == row;
+    } else {
+        for (uint32_t i = 0; i < n; ++i) met |= a.tokens.row(i) == row;
+    }
+    uint64_t clear = __builtin_amdgcn_ballot_w64(!met && row < a.tokens.rows);
+    const float zero[U] = {};
+    for (uint32_t k = 0; clear; ++k, clear &= clear - 1) {
+        if (k % waves != wave) continue;
+        const uint64_t at = static_cast<uint64_t>(first + __builtin_ctzll(clear)) * a.acc_stride;
+        for (uint32_t col = lane * U; col < a.cols; col += kLanes * U) {
+            if (a.cols - col >= U)
+                row_store<AT, U, true>(a.acc, at + col, zero);
+            else
+                row_store_some<AT, U>(a.acc, at + col, zero, a.cols - col);
+        }
+    }
+}
+
+template <int AT>
+__global__ __launch_bounds__(256) void embedding_grad_clear_kernel(GradPass a)
+{
+    clear_rows<AT>(a, blockIdx.x);
+}
+
 // ---- summing runs of equal rows -------------------------------------------------------------------
-// Workgroup (block of 512 columns, group): four wavefronts with per_wave consecutive sorted tokens
-// each, eight columns per lane. A run inside a wavefront goes straight to the accumulator; one that
-// crosses into the next wavefront is joined in LDS by the wavefront it begins in, one that crosses
-// into the next workgroup leaves its parts in head / tail for embedding_grad_join_kernel.
-constexpr int kSumWaves = 4;
-constexpr int kBlockCols = kLanes * kRowUnit;
-constexpr int kAhead = 8;  // gradient rows in flight per wavefront
+// Workgroup (block of 64 units of columns, group): eight wavefronts with per_wave consecutive sorted
+// tokens each, one unit of columns per lane. A run inside a wavefront goes straight to the accumulator; one
+// that crosses into the next wavefront is joined in LDS by the wavefront it begins in; one that crosses
+// workgroups leaves its parts in memory (tail: where it begins, head: in the others) for
+// embedding_grad_join_kernel. (Having the workgroup that delivers a run's last part add them up took longer than the
+// second launch: 38 us against 30 + 4 for 8,192 tokens x 4096.)
+constexpr int kSumWaves = 8;
+
+// Gradient rows in flight per wavefront; the accumulator rows of the runs that end among them are
+// fetched with them, so that a wavefront waits once for all of them and not once per run.
+constexpr int kAhead = 4;
 
 template <int GT, int AT, bool DROP>
 __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(GradPass a)
 {
-    __shared__ float parts[kSumWaves][2][kRowUnit][kLanes];  // 0: head, 1: tail
+    constexpr int U = row_unit<GT, AT>();
+    __shared__ float parts[kSumWaves][2][U][kLanes];               // 0: head, 1: tail
     __shared__ uint32_t head_row[kSumWaves], tail_row[kSumWaves];  // kNoRow: none
     __shared__ uint32_t through[kSumWaves];                        // the head goes on behind the wavefront's end
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n = a.tokens.n, rows = a.tokens.rows;
-    const uint32_t blocks = a.padded / kBlockCols;
-    const uint32_t group = blockIdx.x / blocks;
-    const uint32_t col = ((blockIdx.x - group * blocks) * kLanes + lane) * kRowUnit;
-    const uint32_t count = col >= a.cols ? 0 : (a.cols - col < kRowUnit ? a.cols - col : kRowUnit);
+    const uint32_t blocks = a.padded / (kLanes * U);
+    // A gradient that is written, not added: workgroups behind those of the sums clear rows. (In front of them the
+    // launch took 101 us instead of 82, spread among them 89, as a launch of their own 100: 16,384 tokens, 32,000 rows
+    // of 4096 bf16 elements.)
+    if (blockIdx.x >= a.groups * blocks) {
+        clear_rows<AT>(a, blockIdx.x - a.groups * blocks);
+        return;
+    }
+    const uint32_t group = blockIdx.x / blocks, block = blockIdx.x - group * blocks;
+    const uint32_t col = (block * kLanes + lane) * U;
+    const uint32_t count = col >= a.cols ? 0 : (a.cols - col < U ? a.cols - col : U);
     const uint64_t base = (static_cast<uint64_t>(group) * kSumWaves + wave) * a.per_wave;
     uint64_t key = 0;
     if constexpr (DROP) key = ftc::dropout_key(a.drop);
@@ -495,48 +731,57 @@ __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(
 
     uint32_t h_row = kNoRow, t_row = kNoRow, thru = 0;
     if (valid) {
-        float sum[kRowUnit] = {};
-        uint32_t row = __builtin_amdgcn_readlane(my_row, 0);
-        bool head = row == prev;  // the run that is being summed began before this wavefront
-        auto flush = [&](uint32_t r, bool goes_on) {
-            if (head || goes_on) {
-                const int slot = head ? 0 : 1;
+        const uint32_t first_row = __builtin_amdgcn_readlane(my_row, 0);
+        const bool came_in = first_row == prev;  // the first run began before this wavefront
+        float sum[U] = {};
+        auto keep_part = [&](int slot) {
 #pragma unroll
-                for (int j = 0; j < kRowUnit; ++j) parts[wave][slot][j][lane] = sum[j];
-                if (head) {
-                    h_row = r;
-                    thru = goes_on;
-                } else {
-                    t_row = r;
-                }
-            } else if (count) {
-                finish_unit<AT>(a, r, col, count, sum);
-            }
-            head = false;
+            for (int j = 0; j < U; ++j) parts[wave][slot][j][lane] = sum[j];
         };
         for (uint32_t j0 = 0; j0 < valid; j0 += kAhead) {
-            RowBits<GT> bits[kAhead];
-            uint32_t pos[kAhead], r[kAhead];
+            RowBits<GT, U> bits[kAhead];
+            RowBits<AT, U> old[kAhead];
+            uint32_t pos[kAhead], r[kAhead + 1];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 const uint32_t at = j0 + j < valid ? j0 + j : valid - 1;
                 pos[j] = __builtin_amdgcn_readlane(my_pos, at);
                 r[j] = __builtin_amdgcn_readlane(my_row, at);
-                if (j0 + j < valid && count) bits[j] = load_unit<GT>(a, pos[j], col, count);
+                if (j0 + j < valid && count) bits[j] = load_unit<GT, U, true>(a.g, static_cast<uint64_t>(pos[j]) * a.g_stride + col, count);
+            }
+            r[kAhead] = j0 + kAhead < valid ? __builtin_amdgcn_readlane(my_row, j0 + kAhead) : next;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const uint32_t behind = j0 + j + 1 < valid ? r[j + 1] : next;
+                if (j0 + j < valid && behind != r[j] && !(came_in && r[j] == first_row) && count) old[j] = load_old<AT, U>(a, r[j], col, count);
             }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 if (j0 + j >= valid) break;
-                if (r[j] != row) {
-                    flush(row, false);
-                    row = r[j];
-#pragma unroll
-                    for (int e = 0; e < kRowUnit; ++e) sum[e] = 0.0f;
+                if (count) add_unit<GT, U, DROP>(sum, bits[j], a, key, pos[j], col);
+                const uint32_t behind = j0 + j + 1 < valid ? r[j + 1] : next;
+                if (behind == r[j]) continue;
+                if (came_in && r[j] == first_row) {
+                    keep_part(0);
+                    h_row = first_row;
+                } else if (count) {
+                    finish_unit<AT, U>(a, r[j], col, count, sum, old[j]);
                 }
-                if (count) add_unit<GT, DROP>(sum, bits[j], a, key, pos[j], col);
+#pragma unroll
+                for (int e = 0; e < U; ++e) sum[e] = 0.0f;
             }
         }
-        flush(row, row == next);
+        const uint32_t last = __builtin_amdgcn_readlane(my_row, valid - 1);
+        if (last == next) {  // goes on behind this wavefront
+            if (came_in && last == first_row) {
+                keep_part(0);
+                h_row = last;
+                thru = 1;
+            } else {
+                keep_part(1);
+                t_row = last;
+            }
+        }
     }
     if (lane == 0) {
         head_row[wave] = h_row;
@@ -544,143 +789,169 @@ __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(
         through[wave] = thru;
     }
     __syncthreads();
-    if (!count) return;
-    const uint64_t slot = static_cast<uint64_t>(group) * a.padded + col;
     // The wavefront a run begins in joins it; the one that came in from the workgroup before, wavefront 0.
-    auto join = [&](uint32_t r, uint32_t w, int first_slot, bool goes_on, bool from_before) {
-        float sum[kRowUnit];
+    auto join = [&](uint32_t r, uint32_t w, int slot, bool goes_on, bool from_before) {
+        float sum[U];
 #pragma unroll
-        for (int j = 0; j < kRowUnit; ++j) sum[j] = parts[w][first_slot][j][lane];
+        for (int j = 0; j < U; ++j) sum[j] = parts[w][slot][j][lane];
         while (goes_on && ++w < kSumWaves) {
 #pragma unroll
-            for (int j = 0; j < kRowUnit; ++j) sum[j] += parts[w][0][j][lane];
+            for (int j = 0; j < U; ++j) sum[j] += parts[w][0][j][lane];
             goes_on = through[w];
         }
-        if (from_before || goes_on) {
-            float* to = (from_before ? a.head : a.tail) + slot;
-#pragma unroll
-            for (int j = 0; j < kRowUnit; ++j) to[j] = sum[j];
-        } else {
-            finish_unit<AT>(a, r, col, count, sum);
-        }
+        if (from_before || goes_on)
+            row_store<FT_F32, U, false>(from_before ? a.head : a.tail, static_cast<uint64_t>(group) * a.padded + col, sum);
+        else if (count)
+            finish_unit<AT, U>(a, r, col, count, sum, load_old<AT, U>(a, r, col, count));
     };
     if (wave == 0 && head_row[0] != kNoRow) join(head_row[0], 0, 0, through[0], true);
     if (tail_row[wave] != kNoRow) join(tail_row[wave], wave, 1, true, false);
 }
 
-// Runs that cross workgroups: the workgroup that a run begins in adds the parts up, each of its four
-// wavefronts a quarter of them.
-template <int AT>
-__global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_join_kernel(GradPass a)
+// Runs that cross workgroups of the sums. Up to kLightParts parts: the wavefront of the workgroup that the
+// run begins in adds them up. More (a token that fills the batch, padding): such a run covers a group whose
+// number is a multiple of kLightParts; the first of these has a workgroup per 256 columns, sixteen wavefronts
+// with their share of the parts each. 1,200 parts of one run took 45 us with four wavefronts.
+constexpr uint32_t kLightParts = 32;
+constexpr int kJoinWaves = 16;
+constexpr int kHeavyUnit = 4;
+constexpr uint32_t kHeavyCols = kLanes * kHeavyUnit;
+
+template <int U, int AHEAD>
+__device__ __forceinline__ void add_parts(float (&sum)[U], const GradPass& a, uint32_t from, uint32_t lo, uint32_t hi, uint32_t col)
 {
-    __shared__ float parts[kSumWaves][kRowUnit][kLanes];
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t blocks = a.padded / kBlockCols;
-    const uint32_t group = blockIdx.x / blocks;
-    const uint64_t per_group = static_cast<uint64_t>(a.per_wave) * kSumWaves;
-    const uint64_t begin = group * per_group, end = begin + per_group;
-    const uint32_t n = a.tokens.n;
-    if (end >= n) return;
-    const uint32_t row = a.row_s[end];
-    if (row >= a.tokens.rows || a.row_s[end - 1] != row) return;
-    if (a.row_s[begin] == row && begin > 0 && a.row_s[begin - 1] == row) return;  // began earlier
-    uint32_t heads = 0;  // groups behind this one that begin inside the run
-    for (uint32_t first = group + 1;; first += kLanes) {
-        const uint64_t at = static_cast<uint64_t>(first + lane) * per_group;
-        const uint64_t in = __builtin_amdgcn_ballot_w64(at < n && a.row_s[at < n ? at : 0] == row);
-        const uint32_t run = ~in ? __builtin_ctzll(~in) : kLanes;
-        heads += run;
-        if (run < kLanes) break;
+    for (uint32_t k0 = lo; k0 < hi; k0 += AHEAD) {
+        RowBits<FT_F32, U> bits[AHEAD];
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k)
+            if (k0 + k < hi) bits[k] = row_load<FT_F32, U, false>(k0 + k == 0 ? a.tail : a.head, static_cast<uint64_t>(from + k0 + k) * a.padded + col);
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k)
+            if (k0 + k < hi) {
+#pragma unroll
+                for (int j = 0; j < U; ++j) sum[j] += bits[k][j];
+            }
     }
-    const uint32_t col = ((blockIdx.x - group * blocks) * kLanes + lane) * kRowUnit;
-    const uint32_t parts_all = heads + 1;  // the tail of this group, then the heads
-    const uint32_t lo = static_cast<uint64_t>(parts_all) * wave / kSumWaves, hi = static_cast<uint64_t>(parts_all) * (wave + 1) / kSumWaves;
-    float sum[kRowUnit] = {};
-#pragma unroll 4
-    for (uint32_t k = lo; k < hi; ++k) {
-        const float* from = (k == 0 ? a.tail : a.head) + static_cast<uint64_t>(group + k) * a.padded + col;
-#pragma unroll
-        for (int j = 0; j < kRowUnit; ++j) sum[j] += from[j];
-    }
-#pragma unroll
-    for (int j = 0; j < kRowUnit; ++j) parts[wave][j][lane] = sum[j];
-    __syncthreads();
-    if (wave != 0 || col >= a.cols) return;
-#pragma unroll
-    for (int w = 1; w < kSumWaves; ++w)
-#pragma unroll
-        for (int j = 0; j < kRowUnit; ++j) sum[j] += parts[w][j][lane];
-    finish_unit<AT>(a, row, col, a.cols - col < kRowUnit ? a.cols - col : kRowUnit, sum);
 }
 
-// ---- rows without a token ----------------------------------------------------------------------
-// A gradient that is written, not added: the other rows become zero. A workgroup owns 64 rows; each
-// lane looks its row up among the tokens (binary search in the sorted ones, all of them in a short
-// call).
-template <int AT>
-__global__ __launch_bounds__(256) void embedding_grad_clear_kernel(GradPass a)
+template <int AT, int U>
+__device__ __forceinline__ void join_light(const GradPass& a, uint32_t group, uint32_t block)
 {
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t n = a.tokens.n, first = blockIdx.x * kLanes, row = first + lane;
-    bool met = false;
-    if (a.row_s) {
-        uint32_t lo = 0, hi = n;  // the first sorted token of a row not below this one
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (a.row_s[mid] < row)
-                lo = mid + 1;
-            else
-                hi = mid;
-        }
-        met = lo < n && a.row_s[lo] == row;
-    } else {
-        for (uint32_t i = 0; i < n; ++i) met |= a.tokens.row(i) == row;
+    const uint32_t lane = threadIdx.x & 63u, rows = a.tokens.rows;
+    const uint64_t n = a.tokens.n, per_group = static_cast<uint64_t>(a.per_wave) * kSumWaves, begin = group * per_group, end = begin + per_group;
+    if (end >= n) return;
+    const uint32_t row = a.row_s[end];
+    if (row >= rows || a.row_s[end - 1] != row) return;
+    if (a.row_s[begin] == row && begin > 0 && a.row_s[begin - 1] == row) return;  // began earlier
+    const uint64_t at = end + lane * per_group;  // the group in which part 1 + lane lies
+    const uint64_t in = __builtin_amdgcn_ballot_w64(at < n && a.row_s[at < n ? at : 0] == row);
+    const uint32_t all = 1 + (~in ? __builtin_ctzll(~in) : kLanes);
+    const uint32_t col = (block * kLanes + lane) * U;
+    if (all > kLightParts || col >= a.cols) return;
+    const uint32_t count = a.cols - col < U ? a.cols - col : U;
+    const RowBits<AT, U> old = load_old<AT, U>(a, row, col, count);
+    float sum[U] = {};
+    add_parts<U, 4>(sum, a, group, 0, all, col);
+    finish_unit<AT, U>(a, row, col, count, sum, old);
+}
+
+// How many of lo + 1 ... hi satisfy `in`, which holds up to some index and for none behind it; 64 at a time.
+template <typename F>
+__device__ __forceinline__ uint32_t count_while(uint32_t lo, uint32_t hi, F in)
+{
+    const uint32_t lane = threadIdx.x & 63u, from = lo;
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + kLanes - 1) / kLanes;
+        const uint64_t at = lo + static_cast<uint64_t>(lane + 1) * step;
+        lo += __builtin_popcountll(__builtin_amdgcn_ballot_w64(at <= hi && in(static_cast<uint32_t>(at)))) * step;
+        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
     }
-    uint64_t clear = __builtin_amdgcn_ballot_w64(!met && row < a.tokens.rows);
-    const float zero[kRowUnit] = {};
-    for (uint32_t k = 0; clear; ++k, clear &= clear - 1) {
-        if ((k & 3u) != wave) continue;
-        const uint64_t at = static_cast<uint64_t>(first + __builtin_ctzll(clear)) * a.acc_stride;
-        for (uint32_t col = lane * kRowUnit; col < a.cols; col += kBlockCols) {
-            if (a.cols - col >= kRowUnit)
-                row_store8<AT, true>(a.acc, at + col, zero);
-            else
-                row_store_some<AT>(a.acc, at + col, zero, a.cols - col);
-        }
+    return lo - from;
+}
+
+template <int AT>
+__device__ __forceinline__ void join_heavy(const GradPass& a, uint32_t group, uint32_t block)
+{
+    constexpr int U = kHeavyUnit;
+    __shared__ float parts[kJoinWaves][U][kLanes];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t per_group = static_cast<uint64_t>(a.per_wave) * kSumWaves, at = group * per_group;
+    const uint32_t row = a.row_s[at];
+    if (row >= a.tokens.rows || a.row_s[at - 1] != row) return;
+    // groups in front of which the run is there already, this one's predecessors first
+    const uint32_t earlier = count_while(0, kLightParts, [&](uint32_t k) { return group > k && a.row_s[(group - k) * per_group - 1] == row; });
+    if (earlier >= kLightParts) return;  // another multiple of kLightParts has it
+    const uint32_t from = group - 1 - earlier;
+    const uint32_t all = 2 + earlier + count_while(0, a.groups - 1 - group, [&](uint32_t k) { return a.row_s[(group + k) * per_group] == row; });
+    if (all <= kLightParts) return;
+    const uint32_t col = (block * kLanes + lane) * U;  // below padded, which is a multiple of kHeavyCols
+    const uint32_t lo = static_cast<uint64_t>(all) * wave / kJoinWaves, hi = static_cast<uint64_t>(all) * (wave + 1) / kJoinWaves;
+    float sum[U] = {};
+    add_parts<U, 16>(sum, a, from, lo, hi, col);
+#pragma unroll
+    for (int j = 0; j < U; ++j) parts[wave][j][lane] = sum[j];
+    __syncthreads();
+    if (wave != 0 || col >= a.cols) return;
+    const uint32_t count = a.cols - col < U ? a.cols - col : U;
+    const RowBits<AT, U> old = load_old<AT, U>(a, row, col, count);
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w)
+#pragma unroll
+        for (int j = 0; j < U; ++j) sum[j] += parts[w][j][lane];
+    finish_unit<AT, U>(a, row, col, count, sum, old);
+}
+
+template <int AT, int U>
+__global__ __launch_bounds__(kJoinWaves * kLanes) void embedding_grad_join_kernel(GradPass a, uint32_t light)
+{
+    if (blockIdx.x < light) {
+        const uint32_t blocks = a.padded / (kLanes * U), item = blockIdx.x * kJoinWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (item < a.groups * blocks) join_light<AT, U>(a, item / blocks, item % blocks);
+    } else {
+        const uint32_t blocks = a.padded / kHeavyCols, item = blockIdx.x - light;
+        join_heavy<AT>(a, (item / blocks + 1) * kLightParts, item % blocks);
     }
 }
 
 // ---- host ---------------------------------------------------------------------------------------
 struct GradPlan {
-    uint32_t digit_bits, passes, tiles;
+    uint32_t digit_bits, passes, tiles, items, rotate;  // tiles 0: sorted in one launch
     uint32_t per_wave, groups, padded;
     size_t off_pos_a, off_row_b, off_pos_b, off_count, off_head, off_tail, bytes;  // row_a at 0
 };
 
-GradPlan plan_grad(uint64_t n, uint64_t rows, uint64_t cols)
+// unit: elements per lane of the call's types (the narrower one where only the size is asked for).
+GradPlan plan_grad(uint64_t n, uint64_t rows, uint64_t cols, uint32_t unit)
 {
     GradPlan p{};
     if (n <= kShortTokens) return p;
     uint32_t bits = 1;
     while (bits < 32 && (rows >> bits) != 0) ++bits;  // values up to `rows`
+    if (n <= kBucketTokens && rows <= kBucketRows) {
+        p.rotate = kBucketBits;
+        bits = bits > kBucketBits ? bits - kBucketBits : 0;
+    } else {
+        p.items = n <= kDirectTiles * 2 * kSortThreads ? 2 : 8;
+        p.tiles = static_cast<uint32_t>((n + p.items * kSortThreads - 1) / (p.items * kSortThreads));
+    }
     p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
-    p.digit_bits = (bits + p.passes - 1) / p.passes;
+    p.digit_bits = p.passes ? (bits + p.passes - 1) / p.passes : 0;
     if (p.digit_bits < 6) p.digit_bits = 6;  // at least one counter for each thread of the scan
-    p.tiles = static_cast<uint32_t>((n + kSortTile - 1) / kSortTile);
-    p.padded = static_cast<uint32_t>((cols + kBlockCols - 1) / kBlockCols * kBlockCols);
+    const uint64_t block_cols = kLanes * unit;
+    p.padded = static_cast<uint32_t>((cols + block_cols - 1) / block_cols * block_cols);
     // enough wavefronts to fill the chip, at most 64 tokens each
-    const uint64_t blocks = p.padded / kBlockCols;
+    const uint64_t blocks = p.padded / block_cols;
     uint64_t per_wave = n * blocks / 8192;
-    per_wave = per_wave < 4 ? 4 : per_wave > 64 ? 64 : per_wave;
+    per_wave = per_wave < 4 ? 4 : per_wave > 16 ? 16 : per_wave;
     p.per_wave = static_cast<uint32_t>(per_wave);
     p.groups = static_cast<uint32_t>((n + per_wave * kSumWaves - 1) / (per_wave * kSumWaves));
     auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
     const size_t list = up(n * 4), part = static_cast<size_t>(p.groups) * p.padded * 4;
     p.off_pos_a = list;
     p.off_row_b = 2 * list;
-    p.off_pos_b = 3 * list;
-    p.off_count = 4 * list;
-    p.off_head = p.off_count + up((static_cast<size_t>(p.tiles) << p.digit_bits) * 4);
+    p.off_pos_b = p.off_row_b + (p.tiles ? list : 0);
+    p.off_count = p.off_pos_b + (p.tiles ? list : 0);
+    p.off_head = p.off_count + (p.tiles ? up((static_cast<size_t>(p.tiles + 1) << p.digit_bits) * 4) : 0);
     p.off_tail = p.off_head + part;
     p.bytes = p.off_tail + part;
     return p;
@@ -705,25 +976,47 @@ int sort_tokens(GradPass& a, const GradPlan& p, char* ws, hipStream_t stream)
     s.digit_bits = p.digit_bits;
     s.passes = p.passes;
     s.tiles = p.tiles;
-    s.count = reinterpret_cast<uint32_t*>(ws + p.off_count);
-    const size_t counters = (static_cast<size_t>(kSortWaves) << p.digit_bits) * 4 + kSortWaves * 4;
-    if (p.tiles == 1) {
+    const size_t counters = (static_cast<size_t>(kSortWaves) << p.digit_bits) * 4;
+    if (p.tiles == 0) {
         s.row_out = row_a;
         s.pos_out = pos_a;
-        const size_t r_count = (a.tokens.n + kSortThreads - 1) / kSortThreads;
-        const size_t lds = counters + 2 * r_count * kSortThreads * 4;
-        const int rc = allow_lds(sort_tile_kernel, lds);
+        auto go = [&](auto items) -> int {
+            constexpr int ITEMS = decltype(items)::value;
+            const size_t lds = counters + ITEMS * kSortThreads * 4;
+            const int rc = allow_lds(sort_buckets_kernel<ITEMS>, lds);
+            if (rc != FT_OK) return rc;
+            hipLaunchKernelGGL(sort_buckets_kernel<ITEMS>, dim3(kBuckets), dim3(kSortThreads), lds, stream, s);
+            FT_HIP(hipGetLastError());
+            return FT_OK;
+        };
+        using std::integral_constant;
+        const uint32_t n = a.tokens.n;
+        const int rc = n <= kSortThreads       ? go(integral_constant<int, 1>{})
+                       : n <= 2 * kSortThreads ? go(integral_constant<int, 2>{})
+                       : n <= 4 * kSortThreads ? go(integral_constant<int, 4>{})
+                       : n <= 8 * kSortThreads ? go(integral_constant<int, 8>{})
+                                               : go(integral_constant<int, 16>{});
         if (rc != FT_OK) return rc;
-        hipLaunchKernelGGL(sort_tile_kernel, dim3(1), dim3(kSortThreads), lds, stream, s);
-        FT_HIP(hipGetLastError());
     } else {
+        s.count = reinterpret_cast<uint32_t*>(ws + p.off_count);
+        s.scanned = p.tiles > kDirectTiles;
         for (uint32_t pass = 0; pass < p.passes; ++pass) {
             s.shift = pass * p.digit_bits;
             s.row_out = pass & 1 ? row_b : row_a;
             s.pos_out = pass & 1 ? pos_b : pos_a;
-            hipLaunchKernelGGL(sort_count_kernel, dim3(p.tiles), dim3(kSortThreads), counters, stream, s);
+            if (p.items == 2)
+                hipLaunchKernelGGL(sort_count_kernel<2>, dim3(p.tiles), dim3(kSortThreads), 0, stream, s);
+            else
+                hipLaunchKernelGGL(sort_count_kernel<8>, dim3(p.tiles), dim3(kSortThreads), 0, stream, s);
             FT_HIP(hipGetLastError());
-            hipLaunchKernelGGL(sort_place_kernel, dim3(p.tiles), dim3(kSortThreads), counters, stream, s);
+            if (s.scanned) {
+                hipLaunchKernelGGL(sort_scan_kernel, dim3((1u << p.digit_bits) / kLanes), dim3(kSortThreads), 0, stream, s);
+                FT_HIP(hipGetLastError());
+            }
+            if (p.items == 2)
+                hipLaunchKernelGGL(sort_place_kernel<2>, dim3(p.tiles), dim3(kSortThreads), counters, stream, s);
+            else
+                hipLaunchKernelGGL(sort_place_kernel<8>, dim3(p.tiles), dim3(kSortThreads), counters, stream, s);
             FT_HIP(hipGetLastError());
             s.row_in = s.row_out;
             s.pos_in = s.pos_out;
@@ -731,12 +1024,14 @@ int sort_tokens(GradPass& a, const GradPlan& p, char* ws, hipStream_t stream)
     }
     a.row_s = s.row_out;
     a.pos_s = s.pos_out;
+    a.rotate = p.rotate;
     return FT_OK;
 }
 
 template <int GT, int AT, bool DROP>
 int launch_grad(GradPass a, const GradPlan& p, char* ws, hipStream_t stream)
 {
+    constexpr int U = row_unit<GT, AT>();
     const bool shorter = a.tokens.n <= kShortTokens;
     if (!shorter) {
         a.head = reinterpret_cast<float*>(ws + p.off_head);
@@ -747,21 +1042,24 @@ int launch_grad(GradPass a, const GradPlan& p, char* ws, hipStream_t stream)
         const int rc = sort_tokens(a, p, ws, stream);
         if (rc != FT_OK) return rc;
     }
-    if (!a.accumulate) {
-        hipLaunchKernelGGL((embedding_grad_clear_kernel<AT>), dim3((a.tokens.rows + kLanes - 1) / kLanes), dim3(256), 0, stream, a);
-        FT_HIP(hipGetLastError());
-    }
-    if (a.tokens.n == 0) return FT_OK;
+    const unsigned clearing = a.accumulate ? 0 : (a.tokens.rows + kLanes - 1) / kLanes;
     if (shorter) {
-        hipLaunchKernelGGL((embedding_grad_short_kernel<GT, AT, DROP>), dim3(a.tokens.n, (a.cols + kBlockCols - 1) / kBlockCols), dim3(kLanes), 0,
+        if (clearing) {
+            hipLaunchKernelGGL((embedding_grad_clear_kernel<AT>), dim3(clearing), dim3(256), 0, stream, a);
+            FT_HIP(hipGetLastError());
+        }
+        if (a.tokens.n == 0) return FT_OK;
+        hipLaunchKernelGGL((embedding_grad_short_kernel<GT, AT, DROP>), dim3(a.tokens.n, (a.cols + kLanes * U - 1) / (kLanes * U)), dim3(kLanes), 0,
                            stream, a);
         FT_HIP(hipGetLastError());
         return FT_OK;
     }
-    const unsigned workgroups = p.groups * (p.padded / kBlockCols);
-    hipLaunchKernelGGL((embedding_grad_sum_kernel<GT, AT, DROP>), dim3(workgroups), dim3(kSumWaves * kLanes), 0, stream, a);
+    const unsigned workgroups = p.groups * (p.padded / (kLanes * U));
+    hipLaunchKernelGGL((embedding_grad_sum_kernel<GT, AT, DROP>), dim3(workgroups + clearing), dim3(kSumWaves * kLanes), 0, stream, a);
     FT_HIP(hipGetLastError());
-    hipLaunchKernelGGL((embedding_grad_join_kernel<AT>), dim3(workgroups), dim3(kSumWaves * kLanes), 0, stream, a);
+    const unsigned light = (workgroups + kJoinWaves - 1) / kJoinWaves;
+    const unsigned heavy = (p.groups - 1) / kLightParts * (p.padded / kHeavyCols);  // groups kLightParts, 2 kLightParts, ... below p.groups
+    hipLaunchKernelGGL((embedding_grad_join_kernel<AT, U>), dim3(light + heavy), dim3(kJoinWaves * kLanes), 0, stream, a, light);
     FT_HIP(hipGetLastError());
     return FT_OK;
 }
@@ -839,7 +1137,8 @@ int ft_embedding_lookup(const ft_tokens_t* tokens, const void* table, int table_
 size_t ft_embedding_grad_workspace_bytes(size_t n_tokens, size_t rows, size_t cols)
 {
     if (n_tokens > kMaxCount || rows > kMaxCount || cols > kMaxCols) return 0;  // the call refuses these
-    return plan_grad(n_tokens, rows, cols).bytes;
+    const size_t a = plan_grad(n_tokens, rows, cols, 4).bytes, b = plan_grad(n_tokens, rows, cols, 8).bytes;
+    return a > b ? a : b;
 }
 
 int ft_embedding_grad(const ft_tokens_t* tokens, const void* g, int g_dtype, size_t g_stride, void* acc, int acc_dtype, size_t rows,
@@ -858,12 +1157,14 @@ int ft_embedding_grad(const ft_tokens_t* tokens, const void* g, int g_dtype, siz
         if (rc != FT_OK) return rc;
         a.factor = a.drop.factor;
     }
-    const GradPlan plan = plan_grad(a.tokens.n, rows, cols);
+    const uint32_t unit = g_dtype == FT_F32 || acc_dtype == FT_F32 ? 4 : 8;  // row_unit
+    const GradPlan plan = plan_grad(a.tokens.n, rows, cols, unit);
+    const size_t need = ft_embedding_grad_workspace_bytes(a.tokens.n, rows, cols);
     if (rows == 0 || cols == 0 || (a.tokens.n == 0 && accumulate)) return FT_OK;
-    if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
-        return fth::fail(FT_EINVAL, "the workspace holds %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, plan.bytes);
-    if (plan.bytes && reinterpret_cast<uintptr_t>(workspace) % 16) return fth::fail(FT_EALIGN, "the workspace is not aligned to 16 bytes");
-    if (static_cast<uint64_t>(plan.groups) * (plan.padded / kBlockCols) > 0xffffffull)
+    if (need && (!workspace || workspace_bytes < need))
+        return fth::fail(FT_EINVAL, "the workspace holds %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
+    if (need && reinterpret_cast<uintptr_t>(workspace) % 16) return fth::fail(FT_EALIGN, "the workspace is not aligned to 16 bytes");
+    if (static_cast<uint64_t>(plan.groups) * (plan.padded / (kLanes * unit)) + (accumulate ? 0 : rows / kLanes + 1) > 0xffffffull)
         return fth::fail(FT_EINVAL, "%u tokens of %zu elements are too many for one call", a.tokens.n, cols);
     a.g = g;
     a.acc = acc;

@@ -145,8 +145,8 @@ def test_gradient_types(cuda, g_dtype, acc_dtype, n, p):
     _check_grad(got, acc, tokens, grads, **kw)
 
 
-# around the limits of the variants: 128 tokens without sorting, tiles of 8192, runs of 16 ... 256 tokens
-@pytest.mark.parametrize("n", [0, 1, 2, 63, 64, 65, 127, 128, 129, 1023, 1024, 1025, 8191, 8192, 8193, 16384, 20011])
+# around the limits of the variants: 128 tokens without sorting, 16384 sorted in one launch
+@pytest.mark.parametrize("n", [0, 1, 2, 63, 64, 65, 127, 128, 129, 1023, 1024, 1025, 8191, 8192, 8193, 16383, 16384, 16385, 20011])
 @pytest.mark.parametrize("rows", [1, 2, 63, 64, 65, 511, 512, 513, 50257])
 @pytest.mark.parametrize("accumulate", [True, False])
 def test_gradient_counts(cuda, n, rows, accumulate):
@@ -176,6 +176,20 @@ def test_gradient_runs(cuda, n, how):
     acc, grads = torch.zeros((rows, cols), device=cuda), _randn(cuda, (n, cols), F32, 1)
     got = embedding_grad_(acc.clone(), tokens, grads)
     _check_grad(got, acc, tokens, grads)
+
+
+@pytest.mark.parametrize("n,rows", [(131072, 70000), (131073, 300), (524288, 1 << 19), (524289, 200000), (1 << 20, 40), (5000, (1 << 26) + 5),
+                                    (16384, 1 << 26), (16384, (1 << 17) + 1), (300, 1 << 17)])
+@pytest.mark.parametrize("how", ["frequent and rare", "one and others", "last rows"])
+def test_gradient_sorting(cuda, n, rows, how):
+    """Tiles that are counted directly and by a scan, digits of one, two and three passes, heavy buckets."""
+    i = torch.arange(n, device=cuda)
+    tokens = {"frequent and rare": _ids(cuda, (n,), rows), "one and others": torch.where(i % 4 == 0, i * 7919 % rows, rows // 3),
+              "last rows": rows - 1 - i % 33}[how]
+    grads = torch.randint(-8, 9, (n, 2), device=cuda, generator=_gen(cuda, 2)).to(BF16)  # sums without rounding
+    want = torch.zeros((rows, 2)).index_add_(0, tokens.cpu(), grads.float().cpu())
+    got = embedding_grad_(torch.empty((rows, 2), device=cuda), tokens, grads, accumulate=False)
+    assert torch.equal(got.cpu(), want)
 
 
 def test_gradient_of_whole_numbers_is_exact(cuda):
