@@ -172,7 +172,9 @@ _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 def current_stream_ptr(device=None) -> int:
     """Handle of torch's current stream on ``device`` (default: the current device)."""
     if _RAW_STREAM is not None:  # the same handle without building a Stream object (2 us -> 0.3 us)
-        if device is None:
+        if isinstance(device, int):
+            index = device
+        elif device is None:
             index = torch.cuda.current_device()
         else:
             index = device.index if isinstance(device, torch.device) else torch.device(device).index

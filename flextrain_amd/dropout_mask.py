@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 
 from . import _C
-from .rows import Seed, dropout_record, on_device, require_gpu, row_stride, with_even_rows
+from .rows import Seed, dropout_record, enqueue, gpu_index, row_stride, with_even_rows
 
 
 def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index: int = 0, residual: Optional[Tensor] = None,
@@ -37,24 +37,23 @@ def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index:
 
 def _apply(x: Tensor, p: float, seed: Seed, substream: int, first_index: int, residual: Optional[Tensor] = None, out: Optional[Tensor] = None,
            dtype: Optional[torch.dtype] = None) -> Tensor:
-    require_gpu(x.device, x=x, residual=residual, out=out)
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
+    index = gpu_index(x=x, residual=residual, out=out)
+    shape = x.shape
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(shape)}")
     if dtype is None:
         dtype = x.dtype if residual is None else residual.dtype
     if out is None:
-        out = torch.empty(x.shape, dtype=dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != dtype:
-        raise ValueError(f"out must have shape {tuple(x.shape)} and type {dtype}")
-    cols = x.shape[-1] if x.dim() else 1
+        out = x.new_empty(shape, dtype=dtype)
+    elif out.shape != shape or out.dtype != dtype:
+        raise ValueError(f"out must have shape {tuple(shape)} and type {dtype}")
+    cols = shape[-1] if shape else 1
     rows = x.numel() // cols if cols else 0
-    record = dropout_record(x.device, p, seed, substream, first_index)
-    with on_device(x.device):
-        _C.check("ft_dropout", _C.lib().ft_dropout(
+    enqueue("ft_dropout", _C.lib().ft_dropout, index,
             x.data_ptr(), _C.dtype_code(x.dtype), row_stride("x", x, cols),
             None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride("residual", residual, cols),
-            out.data_ptr(), _C.dtype_code(dtype), row_stride("out", out, cols), rows, cols, ctypes.byref(record),
-            _C.current_stream_ptr(x.device)))
+            out.data_ptr(), _C.dtype_code(dtype), row_stride("out", out, cols), rows, cols,
+            ctypes.byref(dropout_record(index, p, seed, substream, first_index)))
     return out
 
 

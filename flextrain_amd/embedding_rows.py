@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _C
-from .rows import Seed, dropout_record, on_device, require_gpu, row_stride, token_record, with_even_rows
+from .rows import Seed, dropout_record, enqueue, gpu_index, row_stride, token_record, with_even_rows
 
 
 def _table(name: str, t: Tensor) -> int:
@@ -37,20 +37,19 @@ def embedding_lookup(tokens: Tensor, table: Tensor, *, scale: float = 1.0, first
     strides (``batch[:, :-1]``). One fp32 product per element, rounded once. Dropout as in
     ``flextrain_amd.dropout_mask``: element ``i`` of the result is element ``first_index + i`` of
     ``(seed, substream)``."""
-    require_gpu(table.device, table=table, tokens=tokens, out=out)
+    index = gpu_index(table=table, tokens=tokens, out=out)
     table_stride = _table("table", table)
     rows, cols = table.shape
     shape = (*tokens.shape, cols)
     if out is None:
-        out = torch.empty(shape, dtype=table.dtype if dtype is None else dtype, device=table.device)
+        out = table.new_empty(shape, dtype=dtype)
     elif out.shape != shape or (dtype is not None and out.dtype != dtype):
         raise ValueError(f"out must have shape {shape}" + ("" if dtype is None else f" and type {dtype}"))
     record, _ = token_record(tokens, first_row, None)
-    drop = None if dropout == 0.0 else ctypes.byref(dropout_record(table.device, dropout, seed, substream, first_index))
-    with on_device(table.device):
-        _C.check("ft_embedding_lookup", _C.lib().ft_embedding_lookup(
+    enqueue("ft_embedding_lookup", _C.lib().ft_embedding_lookup, index,
             ctypes.byref(record), table.data_ptr(), _C.dtype_code(table.dtype), rows, table_stride, out.data_ptr(), _C.dtype_code(out.dtype),
-            row_stride("out", out, cols), cols, scale, drop, _C.current_stream_ptr(table.device)))
+            row_stride("out", out, cols), cols, scale,
+            None if dropout == 0.0 else ctypes.byref(dropout_record(index, dropout, seed, substream, first_index)))
     return out
 
 
@@ -63,22 +62,20 @@ def embedding_grad_(acc: Tensor, tokens: Tensor, grads: Tensor, *, scale: float 
     in every row without a token. With ``dropout`` the mask of the lookup that had the same values is
     applied to ``grads`` first. Sums are kept in fp32 and rounded to acc's type once; the same call
     gives the same bits."""
-    require_gpu(acc.device, acc=acc, tokens=tokens, grads=grads)
+    index = gpu_index(acc=acc, tokens=tokens, grads=grads)
     acc_stride = _table("acc", acc)
     rows, cols = acc.shape
     if grads.shape != (*tokens.shape, cols):
         raise ValueError(f"grads have shape {tuple(grads.shape)}, tokens {tuple(tokens.shape)} and acc {tuple(acc.shape)}")
     record, n = token_record(tokens, first_row, padding_token)
-    drop = None if dropout == 0.0 else ctypes.byref(dropout_record(acc.device, dropout, seed, substream, first_index))
     lib = _C.lib()
-    grads_stride = row_stride("grads", grads, cols)
-    with on_device(acc.device):
-        need = lib.ft_embedding_grad_workspace_bytes(n, rows, cols)
-        workspace = torch.empty(need, dtype=torch.uint8, device=acc.device) if need else None
-        _C.check("ft_embedding_grad", lib.ft_embedding_grad(
-            ctypes.byref(record), grads.data_ptr(), _C.dtype_code(grads.dtype), grads_stride, acc.data_ptr(), _C.dtype_code(acc.dtype), rows,
-            acc_stride, cols, scale, int(bool(accumulate)), drop, None if workspace is None else workspace.data_ptr(), need,
-            _C.current_stream_ptr(acc.device)))
+    need = lib.ft_embedding_grad_workspace_bytes(n, rows, cols)
+    workspace = torch.empty(need, dtype=torch.uint8, device=acc.device) if need else None
+    enqueue("ft_embedding_grad", lib.ft_embedding_grad, index,
+            ctypes.byref(record), grads.data_ptr(), _C.dtype_code(grads.dtype), row_stride("grads", grads, cols), acc.data_ptr(),
+            _C.dtype_code(acc.dtype), rows, acc_stride, cols, scale, int(bool(accumulate)),
+            None if dropout == 0.0 else ctypes.byref(dropout_record(index, dropout, seed, substream, first_index)),
+            None if workspace is None else workspace.data_ptr(), need)
     return acc
 
 
@@ -91,7 +88,7 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, first_row: 
 
     A ``seed`` in GPU memory, and the tokens, must keep their values until the backward pass has run."""
     if grad_into is not None:
-        require_gpu(weight.device, grad_into=grad_into)
+        gpu_index(weight=weight, grad_into=grad_into)
         if grad_into.shape != weight.shape:
             raise ValueError(f"grad_into has shape {tuple(grad_into.shape)}, weight {tuple(weight.shape)}")
         _table("grad_into", grad_into)

@@ -1,7 +1,6 @@
 """What the row operators (embedding, dropout) share: argument checks and the C structs they fill."""
 from __future__ import annotations
 
-from contextlib import nullcontext
 from typing import Optional, Tuple, Union
 
 import torch
@@ -12,18 +11,32 @@ from . import _C
 #: a seed by value, or one int64 element of GPU memory that the kernels read
 Seed = Union[int, Tensor]
 
-_NO_CONTEXT = nullcontext()
 
 
-def on_device(device: torch.device):
-    """Context in which ``device`` is the current one (nothing to enter where it already is)."""
-    return _NO_CONTEXT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def require_gpu(device: torch.device, **tensors: Optional[Tensor]) -> None:
+def gpu_index(**tensors: Optional[Tensor]) -> int:
+    """The GPU that all of the tensors (those that are not None) are on."""
+    index = None
     for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device != device):
-            raise ValueError(f"{name} must be a tensor on {device if device.type == 'cuda' else 'the GPU'}")
+        if t is None:
+            continue
+        at = t.get_device()
+        if index is None:
+            index = at
+        if at < 0 or at != index:
+            raise ValueError(f"{name} must be a tensor on the GPU" + (f" {index}" if index >= 0 and at >= 0 else ""))
+    return index
+
+
+def enqueue(name: str, fn, index: int, *args) -> None:
+    """Calls the C entry ``fn`` with torch's current stream of GPU ``index`` as its last argument, that
+    GPU being the current one."""
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _C.current_stream_ptr(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _C.current_stream_ptr(index))
+    if rc:
+        _C.check(name, rc)
 
 
 def row_stride(name: str, t: Tensor, cols: int) -> int:
@@ -58,7 +71,7 @@ def with_even_rows(t: Tensor) -> Tensor:
         return t.contiguous()
 
 
-def dropout_record(device: torch.device, p: float, seed: Seed, substream: int, first_index: int) -> "_C.Dropout":
+def dropout_record(index: int, p: float, seed: Seed, substream: int, first_index: int) -> "_C.Dropout":
     if not 0 <= substream < 1 << 32:
         raise ValueError("substream must be a 32-bit number")
     if not 0 <= first_index < 1 << 62:
@@ -66,7 +79,8 @@ def dropout_record(device: torch.device, p: float, seed: Seed, substream: int, f
     if isinstance(seed, Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1:
             raise ValueError("a seed in GPU memory is one int64 element")
-        require_gpu(device, seed=seed)
+        if seed.get_device() != index:
+            raise ValueError(f"seed must be a tensor on the GPU {index}")
         return _C.Dropout(p, 0, seed.data_ptr(), first_index, substream, 0)
     if not 0 <= seed < 1 << 64:
         raise ValueError("seed must be a 64-bit number")
