@@ -8,6 +8,7 @@
 // is added with atomics: the tokens are sorted by row (stably: equal rows keep the order of their
 // positions), every wavefront sums a run of consecutive sorted tokens in registers, and runs that
 // cross the edge of a wavefront or a workgroup are joined in a fixed order.
+#include <atomic>
 #include <type_traits>
 
 #include "ft_counter.hpp"
@@ -810,11 +811,11 @@ __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(
 
 // Runs that cross workgroups of the sums. Up to kLightParts parts: the wavefront of the workgroup that the
 // run begins in adds them up. More (a token that fills the batch, padding): such a run covers a group whose
-// number is a multiple of kLightParts; the first of these has a workgroup per 256 columns, sixteen wavefronts
+// number is a multiple of kLightParts; the first of these has a workgroup per 128 columns, sixteen wavefronts
 // with their share of the parts each. 1,200 parts of one run took 45 us with four wavefronts.
 constexpr uint32_t kLightParts = 32;
 constexpr int kJoinWaves = 16;
-constexpr int kHeavyUnit = 4;
+constexpr int kHeavyUnit = 2;
 constexpr uint32_t kHeavyCols = kLanes * kHeavyUnit;
 
 template <int U, int AHEAD>
@@ -957,10 +958,17 @@ GradPlan plan_grad(uint64_t n, uint64_t rows, uint64_t cols, uint32_t unit)
     return p;
 }
 
-template <typename K>
-int allow_lds(K kernel, size_t bytes)
+// Lets a workgroup of KERNEL have `bytes` of dynamic LDS; the attribute is set once per device.
+template <auto KERNEL>
+int allow_lds(size_t bytes)
 {
-    if (bytes > 65536) FT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    static std::atomic<uint64_t> done{0};  // a bit per device
+    int device = 0;
+    FT_HIP(hipGetDevice(&device));
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return FT_OK;
+    FT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    done.fetch_or(bit, std::memory_order_relaxed);
     return FT_OK;
 }
 
@@ -982,9 +990,12 @@ int sort_tokens(GradPass& a, const GradPlan& p, char* ws, hipStream_t stream)
         s.pos_out = pos_a;
         auto go = [&](auto items) -> int {
             constexpr int ITEMS = decltype(items)::value;
-            const size_t lds = counters + ITEMS * kSortThreads * 4;
-            const int rc = allow_lds(sort_buckets_kernel<ITEMS>, lds);
-            if (rc != FT_OK) return rc;
+            constexpr size_t kList = ITEMS * kSortThreads * 4, kMostCounters = (static_cast<size_t>(kSortWaves) << kMaxDigitBits) * 4;
+            const size_t lds = kList + counters;
+            if constexpr (kList + kMostCounters + sizeof(uint32_t) * (kPairTokens + 64) > 65536) {
+                const int rc = allow_lds<sort_buckets_kernel<ITEMS>>(kList + kMostCounters);
+                if (rc != FT_OK) return rc;
+            }
             hipLaunchKernelGGL(sort_buckets_kernel<ITEMS>, dim3(kBuckets), dim3(kSortThreads), lds, stream, s);
             FT_HIP(hipGetLastError());
             return FT_OK;

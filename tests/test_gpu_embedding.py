@@ -179,7 +179,8 @@ def test_gradient_runs(cuda, n, how):
 
 
 @pytest.mark.parametrize("n,rows", [(131072, 70000), (131073, 300), (524288, 1 << 19), (524289, 200000), (1 << 20, 40), (5000, (1 << 26) + 5),
-                                    (16384, 1 << 26), (16384, (1 << 17) + 1), (300, 1 << 17)])
+                                    (16384, 1 << 26), (16384, (1 << 17) + 1),
+                                    (8192, 1 << 17), (300, 1 << 17)])
 @pytest.mark.parametrize("how", ["frequent and rare", "one and others", "last rows"])
 def test_gradient_sorting(cuda, n, rows, how):
     """Tiles that are counted directly and by a scan, digits of one, two and three passes, heavy buckets."""
