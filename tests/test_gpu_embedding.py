@@ -128,6 +128,26 @@ def test_lookup_far_rows(cuda):
     assert not bool(table[1:5].any()) and not bool(table[rows - 5:rows - 1].any())
 
 
+def test_lookup_far_results(cuda):
+    """Results and gradients of more than 2^32 elements; masks of elements beyond 2^32."""
+    n, cols = (1 << 20) + 77, 4104
+    table, tokens = _randn(cuda, (50, cols), BF16), _ids(cuda, (n,), 50)
+    out = embedding_lookup(tokens, table)
+    for at in (0, 1 << 19, 1 << 20, n - 1):
+        assert torch.equal(out[at], table[tokens[at]])
+    out.zero_()
+    rows = torch.tensor([0, 1 << 19, (1 << 20) - 1, 1 << 20, n - 1], device=cuda)
+    out[rows] = torch.randint(-8, 9, (5, cols), device=cuda, generator=_gen(cuda, 4)).to(BF16)
+    want = torch.zeros((50, cols)).index_add_(0, tokens[rows].cpu(), out[rows].float().cpu())
+    assert torch.equal(embedding_grad_(torch.zeros((50, cols), device=cuda), tokens, out).cpu(), want)
+    keep = torch.stack([ref.kept((cols,), 0.5, 3, first_index=int(r) * cols) for r in rows])
+    want = torch.zeros((50, cols)).index_add_(0, tokens[rows].cpu(), out[rows].float().cpu() * keep.float()) * 2
+    assert torch.equal(embedding_grad_(torch.zeros((50, cols), device=cuda), tokens, out, dropout=0.5, seed=3).cpu(), want)
+    embedding_lookup(tokens, table, dropout=0.5, seed=3, out=out)
+    for k, r in enumerate(rows.tolist()):
+        assert torch.equal(out[r].cpu().float(), (table[tokens[r]].float().cpu() * 2 * keep[k].float()).to(BF16).float())
+
+
 # ---- gradient -------------------------------------------------------------------------------------
 
 
