@@ -343,27 +343,36 @@ __device__ __forceinline__ void load_items(uint32_t (&key)[ITEMS], const SortPas
 // Lanes of the wavefront whose digit is this lane's; `active` lanes only.
 __device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool active)
 {
-    uint64_t m = __builtin_amdgcn_ballot_w64(active);
+    const uint64_t among = __builtin_amdgcn_ballot_w64(active);
+    uint32_t lo = static_cast<uint32_t>(among), hi = static_cast<uint32_t>(among >> 32);
 #pragma unroll
     for (uint32_t b = 0; b < kMaxDigitBits; ++b) {
-        const bool one = digit >> b & 1u;
-        const uint64_t v = __builtin_amdgcn_ballot_w64(one);
-        m &= one ? v : ~v;
+        const uint32_t bit = static_cast<uint32_t>(static_cast<int32_t>(digit << (31 - b)) >> 31);  // all ones or none
+        const uint64_t v = __builtin_amdgcn_ballot_w64(bit != 0);
+        lo &= ~(static_cast<uint32_t>(v) ^ bit);
+        hi &= ~(static_cast<uint32_t>(v >> 32) ^ bit);
     }
-    return m;
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x)
+{
+    // lane permutes inside the vector unit: rows of 16 lanes shifted by 1, 2, 4, 8, then the rows' last lanes handed on
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
 }
 
 // Sum over the threads before this one (1024 threads).
 __device__ __forceinline__ uint32_t exclusive_scan(uint32_t x, uint32_t* wave_sums)
 {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint32_t s = x;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(s, d);
-        if (lane >= d) s += y;
-    }
-    __syncthreads();
+    const uint32_t s = wave_scan(x);
     if (lane == 63) wave_sums[wave] = s;
     __syncthreads();
     uint32_t before = 0;
@@ -380,8 +389,9 @@ __device__ __forceinline__ void rank_items(uint32_t (&rank)[ITEMS], const uint32
                                            uint32_t shift, uint32_t bits, uint32_t* counters)
 {
     const uint32_t lane = threadIdx.x & 63u, bins = 1u << bits;
-    volatile uint32_t* mine = counters + (threadIdx.x >> 6) * bins;
-    for (uint32_t b = lane; b < bins; b += kLanes) mine[b] = 0;
+    uint32_t* share = counters + (threadIdx.x >> 6) * bins;
+    for (uint32_t b = lane * 4; b < bins; b += kLanes * 4) *reinterpret_cast<u32x4*>(share + b) = u32x4{0, 0, 0, 0};
+    volatile uint32_t* mine = share;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
@@ -482,7 +492,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_buckets_kernel(SortPass a)
         if (threadIdx.x >= size) return;
         const uint32_t x = pairs[threadIdx.x];
         uint32_t rank = 0;
-#pragma unroll 8
+#pragma unroll 4
         for (uint32_t j = 0; j < size; j += 4) {
             const u32x4 y = *reinterpret_cast<const u32x4*>(pairs + j);
             rank += (y.x < x) + (y.y < x) + (y.z < x) + (y.w < x);
