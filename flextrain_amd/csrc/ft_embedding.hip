@@ -297,9 +297,11 @@ __global__ __launch_bounds__(kLanes) void embedding_grad_short_kernel(GradPass a
 // Up to 16,384 tokens: one launch, no workgroup waits for another. Workgroup b looks through ALL
 // tokens (sixteen per thread at most), keeps those whose row ends in the byte b, counts those that go
 // in front of them, and sorts its own by the row's other bits in LDS. That is 256 times the reading, all of it
-// from the L2, and takes 6 us where sorting in one workgroup took 23 us (8,192 tokens) and two passes of
-// two launches each 50 us (16,384).
-// More: radix sort by digits of at most nine bits, two launches a pass (count, place).
+// from the L2, and takes 7.5 us where sorting in one workgroup took 23 us (8,192 tokens as text has them), 11 us
+// where the radix sort below took 50 (16,384). What bounds it is the looking through: 60 instructions per token and
+// wavefront.
+// More: radix sort by digits of at most nine bits, two launches a pass (count 4 us, place 8 us: 131,072 tokens),
+// which are little more than the latency of their steps.
 //
 // Ranking inside a workgroup: wavefront w holds 64 * R consecutive items, 64 at a time, and counts them
 // per digit in LDS counters of its own; lanes with the same digit find each other with one ballot per bit
@@ -312,7 +314,8 @@ constexpr uint32_t kBuckets = 1u << kBucketBits;
 constexpr uint32_t kBucketPosBits = 14;
 constexpr uint32_t kBucketTokens = 1u << kBucketPosBits;       // tokens of a one-launch sort
 constexpr uint64_t kBucketRows = 1ull << (32 - kBucketPosBits + kBucketBits);  // its rows: the other bits share 32 with the position
-constexpr uint32_t kPairTokens = 512;                          // up to here a bucket is sorted by comparing all pairs
+constexpr uint32_t kFewTokens = 128;                           // up to here a bucket is sorted by comparing all pairs
+constexpr uint32_t kPairTokens = 512;                          // up to here what is left of it without its most frequent row is
 constexpr uint32_t kDirectTiles = 64;                          // up to here every tile adds up the others' counts itself
 
 struct SortPass {
@@ -381,12 +384,12 @@ __device__ __forceinline__ uint32_t exclusive_scan(uint32_t x, uint32_t* wave_su
     return before + s - x;
 }
 
-// Ranks a tile's items by digit. Item r of lane l of wavefront w is item base + 64 r + l, base = 64 w r_count
-// from the tile's begin; those from n on do not exist. counters[w][digit] ends as the number of the wavefront's
-// items with that digit; rank[] as the number of them in front of each item.
+// Ranks items by digit: a wavefront's are its lanes' keys [0], then their keys [1] ..., `have` of them.
+// counters[w][digit] ends as the number of wavefront w's items with that digit; rank[] as the number of them in
+// front of each item.
 template <int ITEMS>
-__device__ __forceinline__ void rank_items(uint32_t (&rank)[ITEMS], const uint32_t (&key)[ITEMS], uint32_t r_count, uint32_t base, uint32_t n,
-                                           uint32_t shift, uint32_t bits, uint32_t* counters)
+__device__ __forceinline__ void rank_items(uint32_t (&rank)[ITEMS], const uint32_t (&key)[ITEMS], uint32_t have, uint32_t shift, uint32_t bits,
+                                           uint32_t* counters)
 {
     const uint32_t lane = threadIdx.x & 63u, bins = 1u << bits;
     uint32_t* share = counters + (threadIdx.x >> 6) * bins;
@@ -395,8 +398,8 @@ __device__ __forceinline__ void rank_items(uint32_t (&rank)[ITEMS], const uint32
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
-        if (static_cast<uint32_t>(r) < r_count) {  // wave-uniform
-            const bool active = base + r * kLanes + lane < n;
+        if (r * kLanes < have) {  // wave-uniform
+            const bool active = r * kLanes + lane < have;
             const uint32_t digit = key[r] >> shift & (bins - 1);
             const uint64_t same = same_digit(digit, active);
             const uint32_t in_front = __builtin_popcountll(same & ((1ull << lane) - 1));
@@ -434,7 +437,7 @@ template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void sort_buckets_kernel(SortPass a)
 {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-    __shared__ uint32_t kept[kSortWaves], in_front[kSortWaves], wave_sums[kSortWaves];
+    __shared__ uint32_t kept[kSortWaves], in_front[kSortWaves], often_of[kSortWaves], below_of[kSortWaves], wave_sums[kSortWaves];
     __shared__ __attribute__((aligned(16))) uint32_t pairs[kPairTokens + 4];
     const uint32_t n = a.tokens.n, rows = a.tokens.rows, me = blockIdx.x;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -486,37 +489,99 @@ __global__ __launch_bounds__(kSortThreads) void sort_buckets_kernel(SortPass a)
         a.row_out[begin + to] = packed >> kBucketPosBits << kBucketBits | me;
         a.pos_out[begin + to] = packed & (kBucketTokens - 1);
     };
-    if (size <= kPairTokens) {  // packed values are all different: the rank is the number of smaller ones
+    // The rank of packed value x among `m` in pairs[]: they are all different, it is the number of smaller ones.
+    auto rank_among = [&](uint32_t x, uint32_t m) {
+        uint32_t rank = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < m; j += 4) {
+            const u32x4 y = *reinterpret_cast<const u32x4*>(pairs + j);
+            rank += (y.x < x) + (y.y < x) + (y.z < x) + (y.w < x);
+        }
+        return rank;
+    };
+    if (size <= kFewTokens) {
         if (threadIdx.x < size + 4) pairs[threadIdx.x] = threadIdx.x < size ? in_order(threadIdx.x) : 0xffffffffu;
         __syncthreads();
         if (threadIdx.x >= size) return;
         const uint32_t x = pairs[threadIdx.x];
-        uint32_t rank = 0;
-#pragma unroll 4
-        for (uint32_t j = 0; j < size; j += 4) {
-            const u32x4 y = *reinterpret_cast<const u32x4*>(pairs + j);
-            rank += (y.x < x) + (y.y < x) + (y.z < x) + (y.w < x);
-        }
-        write(rank, x);
+        write(rank_among(x, size), x);
         return;
     }
-    const uint32_t r_count = (size + kSortThreads - 1) / kSortThreads, first = wave * kLanes * r_count, bins = 1u << a.digit_bits;
-    uint32_t rank[ITEMS];
+    uint32_t have = __builtin_amdgcn_readfirstlane(kept[wave]), from = wave * per_wave;  // this wavefront's items and their place in the list
 #pragma unroll
-    for (int r = 0; r < ITEMS; ++r) {
-        const uint32_t i = first + r * kLanes + lane;
-        key[r] = static_cast<uint32_t>(r) < r_count && i < size ? in_order(i) : 0;
+    for (int r = 0; r < ITEMS; ++r) key[r] = r * kLanes + lane < have ? list[from + r * kLanes + lane] : 0;
+
+    // A large bucket mostly holds one frequent token and few others. The frequent one's tokens are in order
+    // already; the others, if few enough, are ranked in pairs. Which row is taken for the frequent one only
+    // decides about speed: the most common one of eight samples among 64.
+    {
+        const uint32_t sample = in_order(static_cast<uint32_t>(static_cast<uint64_t>(lane) * size / kLanes)) >> kBucketPosBits;
+        uint32_t often = 0, most = 0;
+#pragma unroll
+        for (uint32_t l = 0; l < kLanes; l += 8) {
+            const uint32_t row = __builtin_amdgcn_readlane(sample, l);
+            const uint32_t alike = __builtin_popcountll(__builtin_amdgcn_ballot_w64(sample == row));
+            often = alike > most ? row : often;
+            most = alike > most ? alike : most;
+        }
+        uint32_t own_often = 0, own_below = 0;
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) {
+            if (r * kLanes < have) {
+                const bool valid = r * kLanes + lane < have;
+                const uint32_t row = key[r] >> kBucketPosBits;
+                own_often += __builtin_popcountll(__builtin_amdgcn_ballot_w64(valid && row == often));
+                own_below += __builtin_popcountll(__builtin_amdgcn_ballot_w64(valid && row < often));
+            }
+        }
+        if (lane == 0) {
+            often_of[wave] = own_often;
+            below_of[wave] = own_below;
+        }
+        __syncthreads();
+        uint32_t often_all = 0, often_before = 0, before_all = 0, below = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWaves; ++w) {
+            often_before += w < wave ? often_of[w] : 0;
+            before_all += w < wave ? shares[w] : 0;
+            often_all += often_of[w];
+            below += below_of[w];
+        }
+        const uint32_t others = __builtin_amdgcn_readfirstlane(size - often_all);
+        if (others <= kPairTokens) {
+            uint32_t others_before = before_all - often_before;
+#pragma unroll
+            for (int r = 0; r < ITEMS; ++r) {
+                if (r * kLanes < have) {
+                    const bool valid = r * kLanes + lane < have, is_often = valid && key[r] >> kBucketPosBits == often, is_other = valid && !is_often;
+                    const uint64_t m_often = __builtin_amdgcn_ballot_w64(is_often), m_other = __builtin_amdgcn_ballot_w64(is_other);
+                    const uint64_t front = (1ull << lane) - 1;
+                    if (is_often) write(below + often_before + __builtin_popcountll(m_often & front), key[r]);
+                    if (is_other) pairs[others_before + __builtin_popcountll(m_other & front)] = key[r];
+                    often_before += __builtin_popcountll(m_often);
+                    others_before += __builtin_popcountll(m_other);
+                }
+            }
+            if (threadIdx.x < 4) pairs[others + threadIdx.x] = 0xffffffffu;
+            __syncthreads();
+            if (threadIdx.x >= others) return;
+            const uint32_t x = pairs[threadIdx.x];
+            write(rank_among(x, others) + (x >> kBucketPosBits > often ? often_all : 0), x);
+            return;
+        }
     }
+    const uint32_t per_wave_later = (size + kSortThreads - 1) / kSortThreads * kLanes, bins = 1u << a.digit_bits;
+    uint32_t rank[ITEMS];
     for (uint32_t pass = 0; pass < a.passes; ++pass) {
         const uint32_t shift = kBucketPosBits + pass * a.digit_bits;
-        rank_items<ITEMS>(rank, key, r_count, first, size, shift, a.digit_bits, counters);
+        rank_items<ITEMS>(rank, key, have, shift, a.digit_bits, counters);
         __syncthreads();
         scan_counters(counters, bins, wave_sums);
         __syncthreads();
         const bool last = pass + 1 == a.passes;
 #pragma unroll
         for (int r = 0; r < ITEMS; ++r) {
-            if (static_cast<uint32_t>(r) < r_count && first + r * kLanes + lane < size) {
+            if (r * kLanes + lane < have) {
                 const uint32_t to = counters[wave * bins + (key[r] >> shift & (bins - 1))] + rank[r];
                 if (last)
                     write(to, key[r]);
@@ -526,17 +591,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_buckets_kernel(SortPass a)
         }
         if (last) return;
         __syncthreads();
+        from = wave * per_wave_later;
+        have = from >= size ? 0 : size - from < per_wave_later ? size - from : per_wave_later;
 #pragma unroll
-        for (int r = 0; r < ITEMS; ++r) {
-            const uint32_t i = first + r * kLanes + lane;
-            if (static_cast<uint32_t>(r) < r_count && i < size) key[r] = list[i];
-        }
+        for (int r = 0; r < ITEMS; ++r) key[r] = r * kLanes + lane < have ? list[from + r * kLanes + lane] : 0;
         __syncthreads();
-    }
-#pragma unroll
-    for (int r = 0; r < ITEMS; ++r) {  // no pass: all of one row
-        const uint32_t i = first + r * kLanes + lane;
-        if (static_cast<uint32_t>(r) < r_count && i < size) write(i, key[r]);
     }
 }
 
@@ -622,7 +681,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortPass a)
             halves[1][digit] = all;
         }
     }
-    rank_items<ITEMS>(rank, key, ITEMS, base, n, a.shift, a.digit_bits, lds);
+    const uint32_t have = base >= n ? 0 : n - base < ITEMS * kLanes ? n - base : ITEMS * kLanes;
+    rank_items<ITEMS>(rank, key, have, a.shift, a.digit_bits, lds);
     __syncthreads();
     if (threadIdx.x < bins && !a.scanned) {
         before += halves[0][threadIdx.x];

@@ -186,13 +186,14 @@ def test_gradient_widths(cuda, cols, n, p):
 
 
 @pytest.mark.parametrize("n", [128, 129, 255, 4096, 8192, 30000, 140001])
-@pytest.mark.parametrize("how", ["one", "two", "ends", "blocks", "all different", "sorted", "reversed"])
+@pytest.mark.parametrize("how", ["one", "two", "ends", "blocks", "all different", "sorted", "reversed", "two in a bucket"])
 def test_gradient_runs(cuda, n, how):
     """Runs that begin and end everywhere: inside a wavefront, across wavefronts and workgroups, across all of them."""
     rows, cols = 150000, 64
     i = torch.arange(n, device=cuda)
     tokens = {"one": torch.full_like(i, 77), "two": torch.where(i % 3 == 0, 5, rows - 1), "ends": torch.where((i == 0) | (i == n - 1), i, 9),
-              "blocks": i * 7 // 1000 * 3, "all different": (i * 7919) % rows, "sorted": i // 5, "reversed": (n - 1 - i) // 33}[how]
+              "blocks": i * 7 // 1000 * 3, "all different": (i * 7919) % rows, "sorted": i // 5, "reversed": (n - 1 - i) // 33,
+              "two in a bucket": torch.where(i % 2 == 0, 512, torch.where(i % 5 == 0, 256 * (i % 400), 1024))}[how]
     acc, grads = torch.zeros((rows, cols), device=cuda), _randn(cuda, (n, cols), F32, 1)
     got = embedding_grad_(acc.clone(), tokens, grads)
     _check_grad(got, acc, tokens, grads)
@@ -201,12 +202,12 @@ def test_gradient_runs(cuda, n, how):
 @pytest.mark.parametrize("n,rows", [(131072, 70000), (131073, 300), (524288, 1 << 19), (524289, 200000), (1 << 20, 40), (5000, (1 << 26) + 5),
                                     (16384, 1 << 26), (16384, (1 << 17) + 1),
                                     (8192, 1 << 17), (300, 1 << 17)])
-@pytest.mark.parametrize("how", ["frequent and rare", "one and others", "last rows"])
+@pytest.mark.parametrize("how", ["frequent and rare", "one and others", "last rows", "one bucket"])
 def test_gradient_sorting(cuda, n, rows, how):
     """Tiles that are counted directly and by a scan, digits of one, two and three passes, heavy buckets."""
     i = torch.arange(n, device=cuda)
     tokens = {"frequent and rare": _ids(cuda, (n,), rows), "one and others": torch.where(i % 4 == 0, i * 7919 % rows, rows // 3),
-              "last rows": rows - 1 - i % 33}[how]
+              "last rows": rows - 1 - i % 33, "one bucket": (i * 31 % 97 * 256 + 5) % rows}[how]
     grads = torch.randint(-8, 9, (n, 2), device=cuda, generator=_gen(cuda, 2)).to(BF16)  # sums without rounding
     want = torch.zeros((rows, 2)).index_add_(0, tokens.cpu(), grads.float().cpu())
     got = embedding_grad_(torch.empty((rows, 2), device=cuda), tokens, grads, accumulate=False)
