@@ -166,6 +166,7 @@ int launch_lookup(LookupPass a, hipStream_t stream)
     };
     using std::integral_constant;
     if (units <= 16) return go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    if (units <= 32) return go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
     // 16,376 rows of 4096 bf16 elements, one / two / four units per lane: 29 / 32 / 32 us; with dropout 45 / 33 / 33 us;
     // 32,768 rows of 8192 fp16 elements into fp32: 268 / 202 / 226 us. Few rows need every wavefront they can get.
     const bool few = static_cast<uint64_t>(a.tokens.n) * ((units + kLanes - 1) / kLanes) < 16384;
