@@ -195,10 +195,16 @@ struct GradPass {
     uint32_t padded;         // columns rounded up to whole blocks
 };
 
-template <int DT, int U, bool NT>
+// RAGGED: rows whose width is no multiple of U, the last unit of a row has `count` elements. Kernels without it
+// have no second way to load a unit, and the loads of several tokens are issued one behind the other; with it the
+// compiler waits for each (128 equal tokens of 4096 elements: 38 us instead of 21).
+template <int DT, int U, bool NT, bool RAGGED>
 __device__ __forceinline__ RowBits<DT, U> load_unit(const void* base, uint64_t at, uint32_t count)
 {
-    return count == U ? row_load<DT, U, NT>(base, at) : row_load_some<DT, U>(base, at, count);
+    if constexpr (RAGGED) {
+        if (count != U) return row_load_some<DT, U>(base, at, count);
+    }
+    return row_load<DT, U, NT>(base, at);
 }
 
 // Adds the gradient's unit of token `pos` at column `col`, masked.
@@ -220,7 +226,7 @@ __device__ __forceinline__ void add_unit(float (&sum)[U], const RowBits<GT, U>& 
 }
 
 // acc[row] = [old +] factor * sum: the one rounding to the accumulator's type.
-template <int AT, int U>
+template <int AT, int U, bool RAGGED>
 __device__ __forceinline__ void finish_unit(const GradPass& a, uint32_t row, uint32_t col, uint32_t count, const float (&sum)[U],
                                             const RowBits<AT, U>& old)
 {
@@ -234,25 +240,31 @@ __device__ __forceinline__ void finish_unit(const GradPass& a, uint32_t row, uin
 #pragma unroll
         for (int j = 0; j < U; ++j) x[j] = sum[j] * a.factor;
     }
-    if (count == U)
-        row_store<AT, U, true>(a.acc, at, x);
-    else
-        row_store_some<AT, U>(a.acc, at, x, count);
+    if constexpr (RAGGED) {
+        if (count != U) {
+            row_store_some<AT, U>(a.acc, at, x, count);
+            return;
+        }
+    }
+    row_store<AT, U, true>(a.acc, at, x);
 }
 
-template <int AT, int U>
+template <int AT, int U, bool RAGGED>
 __device__ __forceinline__ RowBits<AT, U> load_old(const GradPass& a, uint32_t row, uint32_t col, uint32_t count)
 {
     RowBits<AT, U> old{};
-    if (a.accumulate) old = load_unit<AT, U, false>(a.acc, static_cast<uint64_t>(row) * a.acc_stride + col, count);
+    if (a.accumulate) old = load_unit<AT, U, false, RAGGED>(a.acc, static_cast<uint64_t>(row) * a.acc_stride + col, count);
     return old;
 }
 
 // Short calls: one launch without sorting. The wavefront of a token looks through all tokens (two
-// per lane); the first token of a row sums the row's gradients, the others leave.
+// per lane); the first token of a row sums the row's gradients, the others leave. One launch of 3 to 4 us where
+// the three of longer calls take 12 (128 different tokens: 7.5 against 14.5 us a call); a row that has all 128
+// takes 21 us, one wavefront per block of columns adding them up, which is why the limit is not higher.
 constexpr uint32_t kShortTokens = 2 * kLanes;
+constexpr uint32_t kShortAhead = 8;  // gradient rows in flight
 
-template <int GT, int AT, bool DROP>
+template <int GT, int AT, bool DROP, bool RAGGED>
 __global__ __launch_bounds__(kLanes) void embedding_grad_short_kernel(GradPass a)
 {
     constexpr int U = row_unit<GT, AT>();
@@ -267,28 +279,30 @@ __global__ __launch_bounds__(kLanes) void embedding_grad_short_kernel(GradPass a
     const uint32_t col = (blockIdx.y * kLanes + lane) * U;
     if (col >= a.cols) return;
     const uint32_t count = a.cols - col < U ? a.cols - col : U;
-    const RowBits<AT, U> old = load_old<AT, U>(a, mine, col, count);
+    const RowBits<AT, U> old = load_old<AT, U, RAGGED>(a, mine, col, count);
     uint64_t key = 0;
     if constexpr (DROP) key = ftc::dropout_key(a.drop);
     float sum[U] = {};
     while (m0 | m1) {
-        uint32_t pos[4];
-        RowBits<GT, U> bits[4];
-        int have = 0;
+        uint32_t pos[kShortAhead], have = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (!(m0 | m1)) break;
-            pos[j] = m0 ? __builtin_ctzll(m0) : kLanes + __builtin_ctzll(m1);
-            if (m0) m0 &= m0 - 1;
-            else m1 &= m1 - 1;
-            bits[j] = load_unit<GT, U, true>(a.g, static_cast<uint64_t>(pos[j]) * a.g_stride + col, count);
-            have = j + 1;
+        for (uint32_t j = 0; j < kShortAhead; ++j) {  // behind the last token: the last one again
+            const bool more = (m0 | m1) != 0;
+            const uint32_t next = m0 ? __builtin_ctzll(m0) : kLanes + (m1 ? __builtin_ctzll(m1) : 0);
+            pos[j] = more ? next : pos[j ? j - 1 : 0];
+            have += more;
+            m1 = m0 ? m1 : m1 & (m1 - 1);
+            m0 = m0 & (m0 - 1);
         }
+        RowBits<GT, U> bits[kShortAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (uint32_t j = 0; j < kShortAhead; ++j)
+            if (!RAGGED || j < have) bits[j] = load_unit<GT, U, true, RAGGED>(a.g, static_cast<uint64_t>(pos[j]) * a.g_stride + col, count);
+#pragma unroll
+        for (uint32_t j = 0; j < kShortAhead; ++j)
             if (j < have) add_unit<GT, U, DROP>(sum, bits[j], a, key, pos[j], col);
     }
-    finish_unit<AT, U>(a, mine, col, count, sum, old);
+    finish_unit<AT, U, RAGGED>(a, mine, col, count, sum, old);
 }
 
 // ---- sorting the tokens by row ------------------------------------------------------------------
@@ -317,7 +331,10 @@ constexpr uint32_t kBucketTokens = 1u << kBucketPosBits;       // tokens of a on
 constexpr uint64_t kBucketRows = 1ull << (32 - kBucketPosBits + kBucketBits);  // its rows: the other bits share 32 with the position
 constexpr uint32_t kFewTokens = 128;                           // up to here a bucket is sorted by comparing all pairs
 constexpr uint32_t kPairTokens = 512;                          // up to here what is left of it without its most frequent row is
-constexpr uint32_t kDirectTiles = 64;                          // up to here every tile adds up the others' counts itself
+// Radix sort: tiles of two tokens per thread keep more compute units busy (131,073 tokens 46 us a call against 69 with
+// eight, 1,048,576 tokens 146 against 151), tiles of eight have fewer counts to add up (4,194,304: 451 against 463).
+constexpr uint32_t kSmallTileTokens = 1u << 21;
+constexpr uint32_t kDirectTiles = 128;  // up to here every tile adds up the others' counts itself (at the limit as fast as a scan between)
 
 struct SortPass {
     Tokens tokens;
@@ -783,7 +800,7 @@ constexpr int kSumWaves = 8;
 // fetched with them, so that a wavefront waits once for all of them and not once per run.
 constexpr int kAhead = 4;
 
-template <int GT, int AT, bool DROP>
+template <int GT, int AT, bool DROP, bool RAGGED>
 __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(GradPass a)
 {
     constexpr int U = row_unit<GT, AT>();
@@ -803,6 +820,7 @@ __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(
     const uint32_t group = blockIdx.x / blocks, block = blockIdx.x - group * blocks;
     const uint32_t col = (block * kLanes + lane) * U;
     const uint32_t count = col >= a.cols ? 0 : (a.cols - col < U ? a.cols - col : U);
+    const uint32_t from = count ? col : 0;  // lanes behind the row's end read its beginning and store nothing
     const uint64_t base = (static_cast<uint64_t>(group) * kSumWaves + wave) * a.per_wave;
     uint64_t key = 0;
     if constexpr (DROP) key = ftc::dropout_key(a.drop);
@@ -833,25 +851,25 @@ __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(
                 const uint32_t at = j0 + j < valid ? j0 + j : valid - 1;
                 pos[j] = __builtin_amdgcn_readlane(my_pos, at);
                 r[j] = __builtin_amdgcn_readlane(my_row, at);
-                if (j0 + j < valid && count) bits[j] = load_unit<GT, U, true>(a.g, static_cast<uint64_t>(pos[j]) * a.g_stride + col, count);
+                bits[j] = load_unit<GT, U, true, RAGGED>(a.g, static_cast<uint64_t>(pos[j]) * a.g_stride + from, count);
             }
             r[kAhead] = j0 + kAhead < valid ? __builtin_amdgcn_readlane(my_row, j0 + kAhead) : next;
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 const uint32_t behind = j0 + j + 1 < valid ? r[j + 1] : next;
-                if (j0 + j < valid && behind != r[j] && !(came_in && r[j] == first_row) && count) old[j] = load_old<AT, U>(a, r[j], col, count);
+                if (j0 + j < valid && behind != r[j] && !(came_in && r[j] == first_row)) old[j] = load_old<AT, U, RAGGED>(a, r[j], from, count);
             }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 if (j0 + j >= valid) break;
-                if (count) add_unit<GT, U, DROP>(sum, bits[j], a, key, pos[j], col);
+                add_unit<GT, U, DROP>(sum, bits[j], a, key, pos[j], from);
                 const uint32_t behind = j0 + j + 1 < valid ? r[j + 1] : next;
                 if (behind == r[j]) continue;
                 if (came_in && r[j] == first_row) {
                     keep_part(0);
                     h_row = first_row;
                 } else if (count) {
-                    finish_unit<AT, U>(a, r[j], col, count, sum, old[j]);
+                    finish_unit<AT, U, RAGGED>(a, r[j], col, count, sum, old[j]);
                 }
 #pragma unroll
                 for (int e = 0; e < U; ++e) sum[e] = 0.0f;
@@ -888,7 +906,7 @@ __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(
         if (from_before || goes_on)
             row_store<FT_F32, U, false>(from_before ? a.head : a.tail, static_cast<uint64_t>(group) * a.padded + col, sum);
         else if (count)
-            finish_unit<AT, U>(a, r, col, count, sum, load_old<AT, U>(a, r, col, count));
+            finish_unit<AT, U, RAGGED>(a, r, col, count, sum, load_old<AT, U, RAGGED>(a, r, col, count));
     };
     if (wave == 0 && head_row[0] != kNoRow) join(head_row[0], 0, 0, through[0], true);
     if (tail_row[wave] != kNoRow) join(tail_row[wave], wave, 1, true, false);
@@ -935,10 +953,10 @@ __device__ __forceinline__ void join_light(const GradPass& a, uint32_t group, ui
     const uint32_t col = (block * kLanes + lane) * U;
     if (all > kLightParts || col >= a.cols) return;
     const uint32_t count = a.cols - col < U ? a.cols - col : U;
-    const RowBits<AT, U> old = load_old<AT, U>(a, row, col, count);
+    const RowBits<AT, U> old = load_old<AT, U, true>(a, row, col, count);
     float sum[U] = {};
     add_parts<U, 4>(sum, a, group, 0, all, col);
-    finish_unit<AT, U>(a, row, col, count, sum, old);
+    finish_unit<AT, U, true>(a, row, col, count, sum, old);
 }
 
 // How many of lo + 1 ... hi satisfy `in`, which holds up to some index and for none behind it; 64 at a time.
@@ -979,12 +997,12 @@ __device__ __forceinline__ void join_heavy(const GradPass& a, uint32_t group, ui
     __syncthreads();
     if (wave != 0 || col >= a.cols) return;
     const uint32_t count = a.cols - col < U ? a.cols - col : U;
-    const RowBits<AT, U> old = load_old<AT, U>(a, row, col, count);
+    const RowBits<AT, U> old = load_old<AT, U, true>(a, row, col, count);
 #pragma unroll
     for (int w = 1; w < kJoinWaves; ++w)
 #pragma unroll
         for (int j = 0; j < U; ++j) sum[j] += parts[w][j][lane];
-    finish_unit<AT, U>(a, row, col, count, sum, old);
+    finish_unit<AT, U, true>(a, row, col, count, sum, old);
 }
 
 template <int AT, int U>
@@ -1017,7 +1035,7 @@ GradPlan plan_grad(uint64_t n, uint64_t rows, uint64_t cols, uint32_t unit)
         p.rotate = kBucketBits;
         bits = bits > kBucketBits ? bits - kBucketBits : 0;
     } else {
-        p.items = n <= kDirectTiles * 2 * kSortThreads ? 2 : 8;
+        p.items = n <= kSmallTileTokens ? 2 : 8;
         p.tiles = static_cast<uint32_t>((n + p.items * kSortThreads - 1) / (p.items * kSortThreads));
     }
     p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
@@ -1124,7 +1142,7 @@ int sort_tokens(GradPass& a, const GradPlan& p, char* ws, hipStream_t stream)
     return FT_OK;
 }
 
-template <int GT, int AT, bool DROP>
+template <int GT, int AT, bool DROP, bool RAGGED>
 int launch_grad(GradPass a, const GradPlan& p, char* ws, hipStream_t stream)
 {
     constexpr int U = row_unit<GT, AT>();
@@ -1146,13 +1164,13 @@ int launch_grad(GradPass a, const GradPlan& p, char* ws, hipStream_t stream)
             FT_HIP(hipGetLastError());
         }
         if (a.tokens.n == 0) return FT_OK;
-        hipLaunchKernelGGL((embedding_grad_short_kernel<GT, AT, DROP>), dim3(a.tokens.n, (a.cols + kLanes * U - 1) / (kLanes * U)), dim3(kLanes), 0,
+        hipLaunchKernelGGL((embedding_grad_short_kernel<GT, AT, DROP, RAGGED>), dim3(a.tokens.n, (a.cols + kLanes * U - 1) / (kLanes * U)), dim3(kLanes), 0,
                            stream, a);
         FT_HIP(hipGetLastError());
         return FT_OK;
     }
     const unsigned workgroups = p.groups * (p.padded / (kLanes * U));
-    hipLaunchKernelGGL((embedding_grad_sum_kernel<GT, AT, DROP>), dim3(workgroups + clearing), dim3(kSumWaves * kLanes), 0, stream, a);
+    hipLaunchKernelGGL((embedding_grad_sum_kernel<GT, AT, DROP, RAGGED>), dim3(workgroups + clearing), dim3(kSumWaves * kLanes), 0, stream, a);
     FT_HIP(hipGetLastError());
     const unsigned light = (workgroups + kJoinWaves - 1) / kJoinWaves;
     const unsigned heavy = (p.groups - 1) / kLightParts * (p.padded / kHeavyCols);  // groups kLightParts, 2 kLightParts, ... below p.groups
@@ -1276,7 +1294,8 @@ int ft_embedding_grad(const ft_tokens_t* tokens, const void* g, int g_dtype, siz
             constexpr int GT = decltype(gt)::value, AT = decltype(at)::value;
             char* ws = static_cast<char*>(workspace);
             const hipStream_t s = static_cast<hipStream_t>(stream);
-            return masked ? launch_grad<GT, AT, true>(a, plan, ws, s) : launch_grad<GT, AT, false>(a, plan, ws, s);
+            if (cols % row_unit<GT, AT>() != 0) return masked ? launch_grad<GT, AT, true, true>(a, plan, ws, s) : launch_grad<GT, AT, false, true>(a, plan, ws, s);
+            return masked ? launch_grad<GT, AT, true, false>(a, plan, ws, s) : launch_grad<GT, AT, false, false>(a, plan, ws, s);
         });
     });
 }

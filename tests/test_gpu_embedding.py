@@ -176,7 +176,7 @@ def test_gradient_counts(cuda, n, rows, accumulate):
     _check_grad(got, acc, tokens, grads, accumulate=accumulate)
 
 
-@pytest.mark.parametrize("cols", [1, 7, 8, 9, 504, 511, 512, 513, 1003, 1024, 4096, 5001])
+@pytest.mark.parametrize("cols", [1, 4, 7, 8, 9, 12, 100, 504, 511, 512, 513, 1003, 1024, 4096, 5001])
 @pytest.mark.parametrize("n", [90, 1500])
 @pytest.mark.parametrize("p", [0.0, 0.1])
 def test_gradient_widths(cuda, cols, n, p):
@@ -199,7 +199,8 @@ def test_gradient_runs(cuda, n, how):
     _check_grad(got, acc, tokens, grads)
 
 
-@pytest.mark.parametrize("n,rows", [(131072, 70000), (131073, 300), (524288, 1 << 19), (524289, 200000), (1 << 20, 40), (5000, (1 << 26) + 5),
+@pytest.mark.parametrize("n,rows", [(131072, 70000), (131073, 300), (262144, 1 << 19), (262145, 200000), (1 << 20, 40), (1 << 21, 700),
+                                    ((1 << 21) + 1, 50000), (5000, (1 << 26) + 5),
                                     (16384, 1 << 26), (16384, (1 << 17) + 1),
                                     (8192, 1 << 17), (300, 1 << 17)])
 @pytest.mark.parametrize("how", ["frequent and rare", "one and others", "last rows", "one bucket"])
@@ -246,6 +247,35 @@ def test_gradient_skips_padding_and_other_shards(cuda, n):
     for bad in (torch.full_like(tokens, 17), torch.full_like(tokens, -1), torch.full_like(tokens, rows)):  # nothing left
         assert torch.equal(embedding_grad_(acc.clone(), bad, grads, padding_token=17), acc)
         assert not bool(embedding_grad_(acc.clone(), bad, grads, padding_token=17, accumulate=False).any())
+
+
+@pytest.mark.parametrize("n", [60, 3000])
+@pytest.mark.parametrize("g_dtype,acc_dtype", [(BF16, F16), (F16, F32), (F32, BF16)])
+@pytest.mark.parametrize("at", [1, 2, 3, 5])
+def test_rows_at_any_element(cuda, n, g_dtype, acc_dtype, at):
+    """Whole units of rows that begin at any element: all that an address is aligned to is one element."""
+    tokens = _ids(cuda, (n,), 70)
+    grads, store = _randn(cuda, (n, 133), g_dtype)[:, at:at + 128], _randn(cuda, (70, 133), acc_dtype, 1)
+    acc = store[:, at - 1:at + 127]
+    before = store.clone()
+    embedding_grad_(acc, tokens, grads, scale=0.5, dropout=0.1, seed=2)
+    _check_grad(acc, before[:, at - 1:at + 127], tokens, grads, scale=0.5, dropout=0.1, seed=2)
+    assert torch.equal(store[:, :at - 1], before[:, :at - 1]) and torch.equal(store[:, at + 127:], before[:, at + 127:])
+    out = torch.empty((n, 137), device=cuda, dtype=g_dtype)[:, at:at + 128]
+    _check_lookup(embedding_lookup(tokens, acc, out=out, dropout=0.1, seed=2), tokens, acc, dropout=0.1, seed=2)
+
+
+def test_one_token_without_a_dimension(cuda):
+    acc, token, grad = _randn(cuda, (9, 40), F32), torch.tensor(7, device=cuda), _randn(cuda, (40,), F32, 1)
+    _check_grad(embedding_grad_(acc.clone(), token, grad), acc, token, grad)
+
+
+@pytest.mark.parametrize("n", [70, 900])
+def test_everything_dropped(cuda, n):
+    acc, tokens, grads = _randn(cuda, (50, 40), F32), _ids(cuda, (n,), 50), torch.full((n, 40), float("nan"), device=cuda)
+    assert torch.equal(embedding_grad_(acc.clone(), tokens, grads, dropout=1.0, seed=3), acc)
+    assert not bool(embedding_grad_(acc.clone(), tokens, grads, dropout=1.0, seed=3, accumulate=False).any())
+    assert not bool(embedding_lookup(tokens, torch.full_like(acc, float("inf")), dropout=1.0, seed=3).any())
 
 
 @pytest.mark.parametrize("n", [60, 3000])
