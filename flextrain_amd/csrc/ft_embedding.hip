@@ -1035,7 +1035,7 @@ struct GradPlan {
     size_t off_pos_a, off_row_b, off_pos_b, off_count, off_head, off_tail, bytes;  // row_a at 0
 };
 
-// unit: elements per lane of the call's types (the narrower one where only the size is asked for).
+// unit: elements per lane for the call's types (row_unit).
 GradPlan plan_grad(uint64_t n, uint64_t rows, uint64_t cols, uint32_t unit)
 {
     GradPlan p{};
@@ -1051,10 +1051,10 @@ GradPlan plan_grad(uint64_t n, uint64_t rows, uint64_t cols, uint32_t unit)
     }
     p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
     p.digit_bits = p.passes ? (bits + p.passes - 1) / p.passes : 0;
-    if (p.digit_bits < 6) p.digit_bits = 6;  // at least one counter for each thread of the scan
+    if (p.digit_bits < 6) p.digit_bits = 6;  // at least one counter for each thread that scans them
     const uint64_t block_cols = kLanes * unit;
     p.padded = static_cast<uint32_t>((cols + block_cols - 1) / block_cols * block_cols);
-    // enough wavefronts to fill the chip, at most 64 tokens each
+    // enough wavefronts to fill the chip, at most sixteen tokens each (see the sums)
     const uint64_t blocks = p.padded / block_cols;
     uint64_t per_wave = n * blocks / 8192;
     per_wave = per_wave < 4 ? 4 : per_wave > 16 ? 16 : per_wave;

@@ -84,6 +84,11 @@ def test_lookup_token_layouts(cuda, dtype):
                    wide[:, :1].expand(6, 9)):
         got = embedding_lookup(tokens, table)
         assert got.shape == (*tokens.shape, 96) and torch.equal(got, table[tokens.long()])
+        got = embedding_lookup(tokens, table, dropout=0.3, seed=5, first_index=9)
+        _check_lookup(got, tokens, table, dropout=0.3, seed=5, first_index=9)
+        if tokens.numel():
+            grads, acc = _randn(cuda, got.shape, F32, 1), torch.zeros_like(table)
+            _check_grad(embedding_grad_(acc.clone(), tokens, grads, dropout=0.3, seed=5), acc, tokens, grads, dropout=0.3, seed=5)
 
 
 def test_lookup_outside_the_table(cuda):
@@ -202,7 +207,7 @@ def test_gradient_runs(cuda, n, how):
 @pytest.mark.parametrize("n,rows", [(131072, 70000), (131073, 300), (262144, 1 << 19), (262145, 200000), (1 << 20, 40), (1 << 21, 700),
                                     ((1 << 21) + 1, 50000), (5000, (1 << 26) + 5),
                                     (16384, 1 << 26), (16384, (1 << 17) + 1),
-                                    (8192, 1 << 17), (300, 1 << 17)])
+                                    (8192, 1 << 17), (300, 1 << 17), (16384, 100000), (8192, 100000)])
 @pytest.mark.parametrize("how", ["frequent and rare", "one and others", "last rows", "one bucket"])
 def test_gradient_sorting(cuda, n, rows, how):
     """Tiles that are counted directly and by a scan, digits of one, two and three passes, heavy buckets."""
