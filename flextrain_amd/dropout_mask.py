@@ -43,16 +43,18 @@ def _apply(x: Tensor, p: float, seed: Seed, substream: int, first_index: int, re
         raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(shape)}")
     if dtype is None:
         dtype = x.dtype if residual is None else residual.dtype
+    cols = shape[-1] if shape else 1
     if out is None:
-        out = x.new_empty(shape, dtype=dtype)
+        out, out_stride = x.new_empty(shape, dtype=dtype), cols
     elif out.shape != shape or out.dtype != dtype:
         raise ValueError(f"out must have shape {tuple(shape)} and type {dtype}")
-    cols = shape[-1] if shape else 1
+    else:
+        out_stride = row_stride("out", out, cols)
     rows = x.numel() // cols if cols else 0
     enqueue("ft_dropout", _C.lib().ft_dropout, index,
             x.data_ptr(), _C.dtype_code(x.dtype), row_stride("x", x, cols),
             None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride("residual", residual, cols),
-            out.data_ptr(), _C.dtype_code(dtype), row_stride("out", out, cols), rows, cols,
+            out.data_ptr(), _C.dtype_code(dtype), out_stride, rows, cols,
             ctypes.byref(dropout_record(index, p, seed, substream, first_index)))
     return out
 

@@ -42,13 +42,15 @@ def embedding_lookup(tokens: Tensor, table: Tensor, *, scale: float = 1.0, first
     rows, cols = table.shape
     shape = (*tokens.shape, cols)
     if out is None:
-        out = table.new_empty(shape, dtype=dtype)
+        out, out_stride = table.new_empty(shape, dtype=dtype), cols
     elif out.shape != shape or (dtype is not None and out.dtype != dtype):
         raise ValueError(f"out must have shape {shape}" + ("" if dtype is None else f" and type {dtype}"))
+    else:
+        out_stride = row_stride("out", out, cols)
     record, _ = token_record(tokens, first_row, None)
     enqueue("ft_embedding_lookup", _C.lib().ft_embedding_lookup, index,
             ctypes.byref(record), table.data_ptr(), _C.dtype_code(table.dtype), rows, table_stride, out.data_ptr(), _C.dtype_code(out.dtype),
-            row_stride("out", out, cols), cols, scale,
+            out_stride, cols, scale,
             None if dropout == 0.0 else ctypes.byref(dropout_record(index, dropout, seed, substream, first_index)))
     return out
 
