@@ -468,14 +468,17 @@ __global__ __launch_bounds__(kSortThreads) void sort_buckets_kernel(SortPass a)
 
     uint32_t key[ITEMS];
     load_rows<ITEMS>(key, a.tokens, wave * per_wave + lane);
+    // Rotated, a row's bucket is its upper byte and what the bucket is sorted by the rest; kNoRow stays behind all rows.
+    const uint32_t first_of_bucket = me << (32 - kBucketBits);
     uint32_t own = 0, before = 0;
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
-        const bool valid = key[r] != kNoRow;
-        const uint32_t bucket = key[r] & (kBuckets - 1), i = wave * per_wave + r * kLanes + lane;
-        const uint64_t mine = __builtin_amdgcn_ballot_w64(valid && bucket == me);
-        before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(valid && bucket < me));
-        if (valid && bucket == me) list[wave * per_wave + own + __builtin_popcountll(mine & ((1ull << lane) - 1))] = key[r] >> kBucketBits << kBucketPosBits | i;
+        const uint32_t rotated = key[r] >> kBucketBits | key[r] << (32 - kBucketBits), rest = rotated - first_of_bucket;
+        const bool is_mine = rest < (1u << (32 - kBucketPosBits));
+        const uint64_t mine = __builtin_amdgcn_ballot_w64(is_mine);
+        before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(rotated < first_of_bucket));
+        if (is_mine)
+            list[wave * per_wave + own + __builtin_popcountll(mine & ((1ull << lane) - 1))] = rest << kBucketPosBits | (wave * per_wave + r * kLanes + lane);
         own += __builtin_popcountll(mine);
     }
     if (lane == 0) {
