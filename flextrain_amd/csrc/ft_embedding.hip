@@ -260,57 +260,9 @@ __device__ __forceinline__ RowBits<AT, U> load_old(const GradPass& a, uint32_t r
     return old;
 }
 
-// Short calls: one launch without sorting. The wavefront of a token looks through all tokens (two
-// per lane); the first token of a row sums the row's gradients, the others leave. One launch of 3 to 4 us where
-// the three of longer calls take 12 (128 different tokens: 7.5 against 14.5 us a call); a row that has all 128
-// takes 21 us, one wavefront per block of columns adding them up, which is why the limit is not higher.
-constexpr uint32_t kShortTokens = 2 * kLanes;
-constexpr uint32_t kShortAhead = 8;  // gradient rows in flight
-
-template <int GT, int AT, bool DROP, bool RAGGED>
-__global__ __launch_bounds__(kLanes) void embedding_grad_short_kernel(GradPass a)
-{
-    constexpr int U = row_unit<GT, AT>();
-    const uint32_t lane = threadIdx.x, n = a.tokens.n, me = blockIdx.x;
-    const uint32_t r0 = lane < n ? a.tokens.row(lane) : kNoRow;
-    const uint32_t r1 = lane + kLanes < n ? a.tokens.row(lane + kLanes) : kNoRow;
-    const uint32_t mine = __builtin_amdgcn_readlane(me < kLanes ? r0 : r1, me & 63u);
-    if (mine == kNoRow) return;
-    uint64_t m0 = __builtin_amdgcn_ballot_w64(r0 == mine), m1 = __builtin_amdgcn_ballot_w64(r1 == mine);
-    const uint32_t first = m0 ? __builtin_ctzll(m0) : kLanes + __builtin_ctzll(m1);
-    if (first != me) return;
-    const uint32_t col = (blockIdx.y * kLanes + lane) * U;
-    if (col >= a.cols) return;
-    const uint32_t count = a.cols - col < U ? a.cols - col : U;
-    const RowBits<AT, U> old = load_old<AT, U, RAGGED>(a, mine, col, count);
-    uint64_t key = 0;
-    if constexpr (DROP) key = ftc::dropout_key(a.drop);
-    float sum[U] = {};
-    while (m0 | m1) {
-        uint32_t pos[kShortAhead], have = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < kShortAhead; ++j) {  // behind the last token: the last one again
-            const bool more = (m0 | m1) != 0;
-            const uint32_t next = m0 ? __builtin_ctzll(m0) : kLanes + (m1 ? __builtin_ctzll(m1) : 0);
-            pos[j] = more ? next : pos[j ? j - 1 : 0];
-            have += more;
-            m1 = m0 ? m1 : m1 & (m1 - 1);
-            m0 = m0 & (m0 - 1);
-        }
-        RowBits<GT, U> bits[kShortAhead];
-#pragma unroll
-        for (uint32_t j = 0; j < kShortAhead; ++j)
-            if (!RAGGED || j < have) bits[j] = load_unit<GT, U, true, RAGGED>(a.g, static_cast<uint64_t>(pos[j]) * a.g_stride + col, count);
-#pragma unroll
-        for (uint32_t j = 0; j < kShortAhead; ++j)
-            if (j < have) add_unit<GT, U, DROP>(sum, bits[j], a, key, pos[j], col);
-    }
-    finish_unit<AT, U, RAGGED>(a, mine, col, count, sum, old);
-}
-
 // ---- sorting the tokens by row ------------------------------------------------------------------
 // Stable: tokens of one row keep their order, so that sums do not depend on how workgroups run. Which
-// order the rows have among each other does not matter, as long as the clearing kernel knows it.
+// order the rows have among each other does not matter, as long as clear_unmet knows it.
 //
 // Up to 16,384 tokens: one launch, no workgroup waits for another. Workgroup b looks through ALL
 // tokens (sixteen per thread at most), keeps those whose row ends in the byte b, counts those that go
@@ -734,63 +686,184 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortPass a)
 }
 
 // ---- rows without a token ----------------------------------------------------------------------
-// A gradient that is written, not added: the other rows become zero. A workgroup takes kClearRows rows at a
-// time; a lane looks one of them up among the tokens (binary search in the sorted ones, all of them in a short
-// call). 64 rows at a time left the last workgroups alone for longer: 82 us against 77, sums included, for 32,000
-// rows of 4096 bf16 elements.
+// A gradient that is written, not added: the other rows become zero. A workgroup takes kClearRows rows at a time.
+// 64 rows at a time left the last workgroups alone for longer: 82 us against 77, sums included, for 32,000 rows of 4096
+// bf16 elements.
 constexpr uint32_t kClearRows = 16;
 constexpr uint32_t kMostClearing = 1u << 20;  // workgroups of a launch that clear
 
+// Clears the rows first + b of the bits b in `clear`, which are inside the table.
 template <int AT>
-__device__ __forceinline__ void clear_rows(const GradPass& a, uint32_t me, uint32_t of)
+__device__ __forceinline__ void clear_rows(const GradPass& a, uint64_t first, uint64_t clear)
 {
     constexpr int U = AT == FT_F32 ? 4 : 8;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const uint32_t n = a.tokens.n;
-    uint32_t r0 = kNoRow, r1 = kNoRow;
-    if (!a.row_s) {
-        r0 = lane < n ? a.tokens.row(lane) : kNoRow;
-        r1 = lane + kLanes < n ? a.tokens.row(lane + kLanes) : kNoRow;
-    }
-    for (uint64_t first = static_cast<uint64_t>(me) * kClearRows; first < a.tokens.rows; first += static_cast<uint64_t>(of) * kClearRows) {
-        const uint64_t row = first + lane;
-        const bool mine = lane < kClearRows && row < a.tokens.rows;
-        bool met = false;
-        if (a.row_s) {
-            auto order = [&](uint32_t r) { return r >= a.tokens.rows ? kNoRow : (r >> a.rotate) | (a.rotate ? r << (32 - a.rotate) : 0); };
-            const uint32_t want = order(mine ? static_cast<uint32_t>(row) : kNoRow);
-            uint32_t lo = 0, hi = mine ? n : 0;  // the first sorted token of a row not in front of this one
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (order(a.row_s[mid]) < want)
-                    lo = mid + 1;
-                else
-                    hi = mid;
-            }
-            met = mine && lo < n && a.row_s[lo] == row;
-        } else {
-            for (uint32_t i = 0; i < n && i < kLanes; ++i) met |= __builtin_amdgcn_readlane(r0, i) == row;
-            for (uint32_t i = kLanes; i < n; ++i) met |= __builtin_amdgcn_readlane(r1, i - kLanes) == row;
-        }
-        uint64_t clear = __builtin_amdgcn_ballot_w64(mine && !met);
-        const float zero[U] = {};
-        for (uint32_t k = 0; clear; ++k, clear &= clear - 1) {
-            if (k % waves != wave) continue;
-            const uint64_t at = (first + __builtin_ctzll(clear)) * a.acc_stride;
-            for (uint32_t col = lane * U; col < a.cols; col += kLanes * U) {
-                if (a.cols - col >= U)
-                    row_store<AT, U, true>(a.acc, at + col, zero);
-                else
-                    row_store_some<AT, U>(a.acc, at + col, zero, a.cols - col);
-            }
+    const float zero[U] = {};
+    for (uint32_t k = 0; clear; ++k, clear &= clear - 1) {
+        if (k % waves != wave) continue;
+        const uint64_t at = (first + __builtin_ctzll(clear)) * a.acc_stride;
+        for (uint32_t col = lane * U; col < a.cols; col += kLanes * U) {
+            if (a.cols - col >= U)
+                row_store<AT, U, true>(a.acc, at + col, zero);
+            else
+                row_store_some<AT, U>(a.acc, at + col, zero, a.cols - col);
         }
     }
 }
 
+// The workgroup `me` of `of`; a lane looks a row up in the sorted tokens.
 template <int AT>
-__global__ __launch_bounds__(256) void embedding_grad_clear_kernel(GradPass a)
+__device__ __forceinline__ void clear_unmet(const GradPass& a, uint32_t me, uint32_t of)
 {
-    clear_rows<AT>(a, blockIdx.x, gridDim.x);
+    const uint32_t lane = threadIdx.x & 63u, n = a.tokens.n;
+    for (uint64_t first = static_cast<uint64_t>(me) * kClearRows; first < a.tokens.rows; first += static_cast<uint64_t>(of) * kClearRows) {
+        const uint64_t row = first + lane;
+        const bool mine = lane < kClearRows && row < a.tokens.rows;
+        auto order = [&](uint32_t r) { return r >= a.tokens.rows ? kNoRow : (r >> a.rotate) | (a.rotate ? r << (32 - a.rotate) : 0); };
+        const uint32_t want = order(mine ? static_cast<uint32_t>(row) : kNoRow);
+        uint32_t lo = 0, hi = mine ? n : 0;  // the first sorted token of a row not in front of this one
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (order(a.row_s[mid]) < want)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        const bool met = mine && lo < n && a.row_s[lo] == row;
+        clear_rows<AT>(a, first, __builtin_amdgcn_ballot_w64(mine && !met));
+    }
+}
+
+// ---- calls without sorting ----------------------------------------------------------------------
+// Few tokens: one launch. A workgroup has a token and eight blocks of columns (a unit per lane each); its threads look
+// through all tokens and list those of the workgroup's row in order. The workgroups of one row's tokens all have the
+// same list then, and share the row's blocks of columns without a word to each other: of a row with one token every
+// wavefront has a block, of a row with more than eight every workgroup has, with the list dealt to its wavefronts eight
+// tokens at a time and their sums joined in LDS in the wavefronts' order.
+//
+// What bounds it is the latency of its steps: 512 different tokens x 4096 bf16 into fp32 5.2 us and a call every 6.9
+// (the host's side of it), where the three launches of the sorted way take 8.9 and 13.7; 512 as text has them 5.8
+// (10.5), one row that has all 512 12.3 (11.4), for which two wavefronts' loads in flight are not enough (sixteen
+// tokens at a time took longer for text: 6.9). With two tokens per thread 1,024 tokens x 4096 take 10.3 us (sorted
+// 11.3; text 9.8 against 12.0, one row 18 against 15), x 512 4.6 (8.3), but x 8192, two workgroups per token, 22.4
+// (20.6).
+constexpr int kUnsortedThreads = 512;
+constexpr int kUnsortedWaves = kUnsortedThreads / kLanes;
+constexpr uint32_t kUnsortedBlocks = kUnsortedWaves;
+constexpr uint32_t kUnsortedAhead = 8;  // gradient rows in flight
+
+// Tokens per thread of a call that is not sorted; 0: sorted.
+uint32_t unsorted_items(uint64_t n, uint64_t cols, uint32_t unit)
+{
+    if (n <= kUnsortedThreads) return 1;
+    return n <= 2 * kUnsortedThreads && cols <= kUnsortedBlocks * kLanes * unit ? 2 : 0;
+}
+
+template <int GT, int AT, bool DROP, bool RAGGED, int ITEMS>
+__global__ __launch_bounds__(kUnsortedThreads) void embedding_grad_unsorted_kernel(GradPass a, uint32_t sums)
+{
+    constexpr int U = row_unit<GT, AT>();
+    __shared__ uint32_t list[ITEMS * kUnsortedThreads];
+    __shared__ uint32_t found[kUnsortedWaves];
+    __shared__ float parts[kUnsortedWaves][U][kLanes];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n = a.tokens.n, at = wave * ITEMS * kLanes + lane;
+    uint32_t row[ITEMS];
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) row[r] = at + r * kLanes < n ? a.tokens.row(at + r * kLanes) : kNoRow;
+    if (blockIdx.x >= sums) {  // a gradient that is written, not added
+        const uint64_t step = static_cast<uint64_t>(gridDim.x - sums) * kClearRows;
+        for (uint64_t first = static_cast<uint64_t>(blockIdx.x - sums) * kClearRows; first < a.tokens.rows; first += step) {
+            uint32_t met = 0;
+#pragma unroll
+            for (int r = 0; r < ITEMS; ++r)
+                if (row[r] != kNoRow && row[r] - first < kClearRows) met |= 1u << (row[r] - first);
+#pragma unroll
+            for (int d = 1; d < kLanes; d <<= 1) met |= __shfl_xor(met, d);
+            if (lane == 0) found[wave] = met;
+            __syncthreads();
+            met = 0;
+#pragma unroll
+            for (int w = 0; w < kUnsortedWaves; ++w) met |= found[w];
+            __syncthreads();
+            const uint64_t left = a.tokens.rows - first;
+            const uint32_t there = left < kClearRows ? (1u << left) - 1 : (1u << kClearRows) - 1;
+            clear_rows<AT>(a, first, __builtin_amdgcn_readfirstlane(there & ~met));
+        }
+        return;
+    }
+    const uint32_t part = blockIdx.x / n, me = blockIdx.x - part * n;
+    const uint32_t mine = a.tokens.row(me);
+    if (mine == kNoRow) return;
+    uint32_t own = 0;
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) own += __builtin_popcountll(__builtin_amdgcn_ballot_w64(row[r] == mine));
+    if (lane == 0) found[wave] = own;
+    __syncthreads();
+    uint32_t to = 0, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kUnsortedWaves; ++w) {
+        const uint32_t f = __builtin_amdgcn_readfirstlane(found[w]);
+        to += w < wave ? f : 0;
+        total += f;
+    }
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint64_t match = __builtin_amdgcn_ballot_w64(row[r] == mine);
+        if (row[r] == mine) list[to + __builtin_popcountll(match & ((1ull << lane) - 1))] = at + r * kLanes;
+        to += __builtin_popcountll(match);
+    }
+    __syncthreads();
+    const uint32_t blocks = (a.cols + kLanes * U - 1) / (kLanes * U) - part * kUnsortedBlocks;
+    const uint32_t shared = blocks < kUnsortedBlocks ? blocks : kUnsortedBlocks, sharers = total < shared ? total : shared;
+    const uint64_t chosen = __builtin_amdgcn_ballot_w64(lane < sharers && list[lane] == me);
+    if (!chosen) return;
+    const uint32_t rank = __builtin_ctzll(chosen);  // of this token among its row's
+    // Eight tokens or fewer: a wavefront has a block. More: the workgroup has one (as many sharers as blocks), the
+    // wavefronts have their tokens of it.
+    const bool many = total > kUnsortedAhead;
+    const uint32_t block = many ? rank : rank + wave * sharers;
+    const uint32_t col = ((part * kUnsortedBlocks + block) * kLanes + lane) * U;
+    const uint32_t count = block >= shared || col >= a.cols ? 0 : a.cols - col < U ? a.cols - col : U;
+    float sum[U] = {};
+    RowBits<AT, U> old{};
+    if (count) {
+        if (!many || wave == 0) old = load_old<AT, U, RAGGED>(a, mine, col, count);
+        uint64_t key = 0;
+        if constexpr (DROP) key = ftc::dropout_key(a.drop);
+        auto add = [&](auto ahead, uint32_t from) {
+            constexpr uint32_t AHEAD = decltype(ahead)::value;
+            uint32_t pos[AHEAD];
+            RowBits<GT, U> bits[AHEAD];
+#pragma unroll
+            for (uint32_t j = 0; j < AHEAD; ++j) {  // behind the last token: the last one again
+                pos[j] = __builtin_amdgcn_readfirstlane(list[from + j < total ? from + j : total - 1]);
+                if (!RAGGED || from + j < total) bits[j] = load_unit<GT, U, true, RAGGED>(a.g, static_cast<uint64_t>(pos[j]) * a.g_stride + col, count);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < AHEAD; ++j)
+                if (from + j < total) add_unit<GT, U, DROP>(sum, bits[j], a, key, pos[j], col);
+        };
+        if (total == 1)
+            add(std::integral_constant<uint32_t, 1>{}, 0);
+        else
+            for (uint32_t from = many ? wave * kUnsortedAhead : 0; from < total; from += kUnsortedWaves * kUnsortedAhead)
+                add(std::integral_constant<uint32_t, kUnsortedAhead>{}, from);
+    }
+    if (many) {
+        if (wave) {
+#pragma unroll
+            for (int j = 0; j < U; ++j) parts[wave][j][lane] = sum[j];
+        }
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 1; w < kUnsortedWaves; ++w) {
+#pragma unroll
+            for (int j = 0; j < U; ++j) sum[j] += parts[w][j][lane];
+        }
+    }
+    if (count) finish_unit<AT, U, RAGGED>(a, mine, col, count, sum, old);
 }
 
 // ---- summing runs of equal rows -------------------------------------------------------------------
@@ -828,7 +901,7 @@ __global__ __launch_bounds__(kSumWaves * kLanes) void embedding_grad_sum_kernel(
     // launch took 101 us instead of 82, spread among them 89, as a launch of their own 100: 16,384 tokens, 32,000 rows
     // of 4096 bf16 elements.)
     if (blockIdx.x >= a.groups * blocks) {
-        clear_rows<AT>(a, blockIdx.x - a.groups * blocks, gridDim.x - a.groups * blocks);
+        clear_unmet<AT>(a, blockIdx.x - a.groups * blocks, gridDim.x - a.groups * blocks);
         return;
     }
     const uint32_t group = blockIdx.x / blocks, block = blockIdx.x - group * blocks;
@@ -1033,6 +1106,7 @@ __global__ __launch_bounds__(kJoinWaves * kLanes) void embedding_grad_join_kerne
 
 // ---- host ---------------------------------------------------------------------------------------
 struct GradPlan {
+    uint32_t unsorted;                                  // tokens per thread without sorting, 0: sorted
     uint32_t digit_bits, passes, tiles, items, rotate;  // tiles 0: sorted in one launch
     uint32_t per_wave, groups, padded;
     size_t off_pos_a, off_row_b, off_pos_b, off_count, off_head, off_tail, bytes;  // row_a at 0
@@ -1042,7 +1116,8 @@ struct GradPlan {
 GradPlan plan_grad(uint64_t n, uint64_t rows, uint64_t cols, uint32_t unit)
 {
     GradPlan p{};
-    if (n <= kShortTokens) return p;
+    p.unsorted = unsorted_items(n, cols, unit);
+    if (p.unsorted) return p;
     uint32_t bits = 1;
     while (bits < 32 && (rows >> bits) != 0) ++bits;  // values up to `rows`
     if (n <= kBucketTokens && rows <= kBucketRows) {
@@ -1160,29 +1235,25 @@ template <int GT, int AT, bool DROP, bool RAGGED>
 int launch_grad(GradPass a, const GradPlan& p, char* ws, hipStream_t stream)
 {
     constexpr int U = row_unit<GT, AT>();
-    const bool shorter = a.tokens.n <= kShortTokens;
-    if (!shorter) {
-        a.head = reinterpret_cast<float*>(ws + p.off_head);
-        a.tail = reinterpret_cast<float*>(ws + p.off_tail);
-        a.per_wave = p.per_wave;
-        a.groups = p.groups;
-        a.padded = p.padded;
-        const int rc = sort_tokens(a, p, ws, stream);
-        if (rc != FT_OK) return rc;
-    }
     unsigned clearing = a.accumulate ? 0 : (a.tokens.rows + kClearRows - 1) / kClearRows;
     if (clearing > kMostClearing) clearing = kMostClearing;
-    if (shorter) {
-        if (clearing) {
-            hipLaunchKernelGGL((embedding_grad_clear_kernel<AT>), dim3(clearing), dim3(256), 0, stream, a);
+    if (p.unsorted) {
+        const uint32_t sums = a.tokens.n * ((a.cols + kUnsortedBlocks * kLanes * U - 1) / (kUnsortedBlocks * kLanes * U));
+        auto go = [&](auto items) -> int {
+            hipLaunchKernelGGL((embedding_grad_unsorted_kernel<GT, AT, DROP, RAGGED, decltype(items)::value>), dim3(sums + clearing),
+                               dim3(kUnsortedThreads), 0, stream, a, sums);
             FT_HIP(hipGetLastError());
-        }
-        if (a.tokens.n == 0) return FT_OK;
-        hipLaunchKernelGGL((embedding_grad_short_kernel<GT, AT, DROP, RAGGED>), dim3(a.tokens.n, (a.cols + kLanes * U - 1) / (kLanes * U)), dim3(kLanes), 0,
-                           stream, a);
-        FT_HIP(hipGetLastError());
-        return FT_OK;
+            return FT_OK;
+        };
+        return p.unsorted == 1 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
     }
+    a.head = reinterpret_cast<float*>(ws + p.off_head);
+    a.tail = reinterpret_cast<float*>(ws + p.off_tail);
+    a.per_wave = p.per_wave;
+    a.groups = p.groups;
+    a.padded = p.padded;
+    const int rc = sort_tokens(a, p, ws, stream);
+    if (rc != FT_OK) return rc;
     const unsigned workgroups = p.groups * (p.padded / (kLanes * U));
     hipLaunchKernelGGL((embedding_grad_sum_kernel<GT, AT, DROP, RAGGED>), dim3(workgroups + clearing), dim3(kSumWaves * kLanes), 0, stream, a);
     FT_HIP(hipGetLastError());

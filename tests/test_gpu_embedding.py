@@ -170,7 +170,7 @@ def test_gradient_types(cuda, g_dtype, acc_dtype, n, p):
     _check_grad(got, acc, tokens, grads, **kw)
 
 
-# around the limits of the variants: 128 tokens without sorting, 16384 sorted in one launch
+# around the limits of the variants: 1024 tokens of such rows without sorting, 16384 sorted in one launch
 @pytest.mark.parametrize("n", [0, 1, 2, 63, 64, 65, 127, 128, 129, 1023, 1024, 1025, 8191, 8192, 8193, 16383, 16384, 16385, 20011])
 @pytest.mark.parametrize("rows", [1, 2, 63, 64, 65, 511, 512, 513, 50257])
 @pytest.mark.parametrize("accumulate", [True, False])
@@ -218,6 +218,38 @@ def test_gradient_sorting(cuda, n, rows, how):
     want = torch.zeros((rows, 2)).index_add_(0, tokens.cpu(), grads.float().cpu())
     got = embedding_grad_(torch.empty((rows, 2), device=cuda), tokens, grads, accumulate=False)
     assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("n", [2, 7, 8, 9, 65, 511, 512, 513, 1023, 1024])
+@pytest.mark.parametrize("cols", [5, 513, 2048, 2049, 4096, 4104, 9001])
+@pytest.mark.parametrize("how", ["one", "eight and nine", "different", "few left"])
+def test_gradient_without_sorting(cuda, n, cols, how):
+    """Rows that one workgroup, some or all of its tokens' workgroups share, in one pass over the columns or several."""
+    rows, i = 1500, torch.arange(n, device=cuda)
+    tokens = {"one": torch.full_like(i, rows - 1), "eight and nine": torch.where(i % 17 < 8, i // 17 * 2, i // 17 * 2 + 1) % rows,
+              "different": (i * 7) % rows, "few left": torch.where(i % 50 == 1, 3, 2000)}[how]
+    for g_dtype, acc_dtype in ((BF16, F32), (F16, BF16)):
+        grads = torch.randint(-8, 9, (n, cols), device=cuda, generator=_gen(cuda, 2)).to(g_dtype)
+        acc = torch.randint(-8, 9, (rows, cols), device=cuda, generator=_gen(cuda, 3)).to(acc_dtype)
+        inside = tokens < rows
+        for accumulate in (True, False):
+            # whole numbers below 2^24: the sum has no rounding, the result's type has one
+            want = acc.double().cpu() if accumulate else torch.zeros((rows, cols), dtype=torch.float64)
+            want.index_add_(0, tokens[inside].cpu(), grads[inside].double().cpu())
+            got = embedding_grad_(acc.clone() if accumulate else torch.full_like(acc, float("nan")), tokens, grads, accumulate=accumulate)
+            assert torch.equal(got.cpu(), want.to(acc_dtype)), (g_dtype, acc_dtype, accumulate)
+
+
+@pytest.mark.parametrize("n,cols", [(512, 700), (1000, 4090), (300, 9000)])
+@pytest.mark.parametrize("g_dtype,acc_dtype", [(BF16, F32), (F32, F32), (F16, F16)])
+def test_masked_gradient_without_sorting(cuda, n, cols, g_dtype, acc_dtype):
+    tokens = _ids(cuda, (n,), 40, 5)
+    tokens[::3] = 39
+    acc, grads = _randn(cuda, (40, cols), acc_dtype), _randn(cuda, (n, cols), g_dtype, 1)
+    kw = dict(scale=0.5, dropout=0.3, seed=8, substream=2, first_index=7, padding_token=3)
+    got = embedding_grad_(acc.clone(), tokens, grads, **kw)
+    _check_grad(got, acc, tokens, grads, **kw)
+    assert torch.equal(embedding_grad_(acc.clone(), tokens, grads, **kw), got)
 
 
 def test_gradient_of_whole_numbers_is_exact(cuda):
