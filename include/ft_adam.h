@@ -400,7 +400,8 @@ int ft_embedding_grad(const ft_tokens_t* tokens, const void* g, int g_dtype, siz
                       size_t workspace_bytes, void* stream);
 
 /* ---- dropout -----------------------------------------------------------------------------------
- * out = [residual +] dropout(x) for rows x cols elements (see ft_dropout_t above). residual (NULL: none)
+ * out = [residual +] dropout(x) for rows x cols elements (see ft_dropout_t above); the product is rounded to fp32,
+ * the sum to fp32 and to out's type. residual (NULL: none)
  * has out's type; out may be x or residual itself where type and strides agree. A dropped element
  * contributes 0, whatever x holds there. The gradient of x is the same call on the gradient of out,
  * without residual; that of residual is the gradient of out. No counterpart in the reference, whose
