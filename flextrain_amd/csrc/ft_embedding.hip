@@ -228,20 +228,22 @@ __device__ __forceinline__ void add_unit(float (&sum)[U], const RowBits<GT, U>& 
     }
 }
 
-// acc[row] = [old +] factor * sum: the one rounding to the accumulator's type.
+// acc[row] = [old +] factor * sum: the one rounding to the accumulator's type. The product is rounded to fp32 before the
+// addition, as a gradient that is written and then added is: a fused multiply-add would keep the rounding of the factor, and
+// sums on the border between two 16-bit numbers would all go to the same side.
 template <int AT, int U, bool RAGGED>
 __device__ __forceinline__ void finish_unit(const GradPass& a, uint32_t row, uint32_t col, uint32_t count, const float (&sum)[U],
                                             const RowBits<AT, U>& old)
 {
     const uint64_t at = static_cast<uint64_t>(row) * a.acc_stride + col;
     float x[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) x[j] = sum[j] * a.factor;
     if (a.accumulate) {
-        row_floats<AT, U>(x, old);
+        float before[U];
+        row_floats<AT, U>(before, old);
 #pragma unroll
-        for (int j = 0; j < U; ++j) x[j] = __builtin_fmaf(sum[j], a.factor, x[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < U; ++j) x[j] = sum[j] * a.factor;
+        for (int j = 0; j < U; ++j) x[j] = before[j] + x[j];
     }
     if constexpr (RAGGED) {
         if (count != U) {

@@ -390,8 +390,8 @@ int ft_embedding_lookup(const ft_tokens_t* tokens, const void* table, int table_
 /* ft_embedding_grad: the lookup's gradient. g holds one row per token; acc[v][c] += scale * the sum of
  * g[i][c] over the tokens i of row v that are no padding (accumulate != 0; other rows are not touched),
  * or acc = that sum with zeros in the rows without a token (accumulate == 0). drop: the lookup's. Sums
- * are kept in fp32 and rounded to acc's type once. Tokens are sorted and added in an order that
- * depends on the arguments alone: the same call gives the same bits.
+ * are kept in fp32, multiplied in fp32, added to acc in fp32 and rounded to its type once. Tokens are
+ * sorted and added in an order that depends on the arguments alone: the same call gives the same bits.
  * workspace: ft_embedding_grad_workspace_bytes(outer * inner, rows, cols) bytes of device memory,
  * 16-byte aligned, which calls that may overlap in time must not share (0 for few tokens: NULL will do). */
 size_t ft_embedding_grad_workspace_bytes(size_t n_tokens, size_t rows, size_t cols);

@@ -39,3 +39,27 @@ def test_what_cancels_is_zero(cuda, dtype):
     keep = ref.kept(x.shape, 0.1, 3) > 0
     want = torch.where(keep, 0.0, -10.0).to(dtype)
     assert torch.equal(dropout(x, 0.1, 3, residual=residual).cpu(), want)
+
+
+@pytest.mark.parametrize("n", [100, 700, 3000, 40000])
+@pytest.mark.parametrize("g_dtype", TYPES)
+def test_accumulated_gradient_is_the_written_one_added(cuda, n, g_dtype):
+    rows, cols = 900, 264
+    tokens = torch.randint(0, rows, (n,), device=cuda, generator=torch.Generator(device=cuda).manual_seed(1))
+    acc, grads = _randn(cuda, (rows, cols), F32), _randn(cuda, (n, cols), g_dtype, 1)
+    kw = dict(scale=0.7, dropout=0.1, seed=4)
+    written = embedding_grad_(torch.empty_like(acc), tokens, grads, accumulate=False, **kw)
+    assert torch.equal(embedding_grad_(acc.clone(), tokens, grads, **kw), acc + written)
+
+
+@pytest.mark.parametrize("n", [100, 700, 3000, 40000])
+@pytest.mark.parametrize("cols", [40, 41])
+@pytest.mark.parametrize("g_dtype", TYPES)
+@pytest.mark.parametrize("acc_dtype", TYPES)
+def test_a_gradient_that_cancels_is_zero(cuda, n, cols, g_dtype, acc_dtype):
+    """Rows with ten tokens, nine of them 1: the sum is 9, times 10 / 9 is 10."""
+    tokens = torch.arange(n, device=cuda) % (n // 10)
+    grads = torch.full((n, cols), 1.0, device=cuda, dtype=g_dtype)
+    grads[:n // 10] = 0.0
+    acc = torch.full((n // 10, cols), -10.0, device=cuda, dtype=acc_dtype)
+    assert not bool(embedding_grad_(acc, tokens, grads, scale=10.0 / 9.0).any())
