@@ -24,6 +24,7 @@ constexpr int kLanes = 64;
 constexpr uint32_t kNoRow = 0xffffffffu;
 constexpr uint64_t kMaxCount = 0x7fffffffull;  // tokens of a call, rows of a table
 constexpr uint64_t kMaxCols = 1ull << 24;      // elements of a row
+constexpr uint64_t kMaxReach = 1ull << 38;     // ids from the first to the last token of either dimension: more than the memory holds
 
 // Token i of a call: id at outer index i / inner, inner index i % inner.
 struct Tokens {
@@ -1274,7 +1275,8 @@ int check_tokens(const ft_tokens_t* t, size_t rows, Tokens* out)
     if (rows > kMaxCount) return fth::fail(FT_EINVAL, "a table has at most 2^31 - 1 rows");
     if (t->outer > kMaxCount || t->inner > kMaxCount || t->outer * t->inner > kMaxCount)
         return fth::fail(FT_EINVAL, "a call takes at most 2^31 - 1 tokens");
-    if (t->outer_stride > ftr::kMaxElements >> 31 || t->inner_stride > ftr::kMaxElements >> 31) return fth::fail(FT_EINVAL, "token strides are too large");
+    auto reaches_too_far = [](uint64_t count, uint64_t stride) { return stride > kMaxReach / (count ? count : 1); };
+    if (reaches_too_far(t->outer, t->outer_stride) || reaches_too_far(t->inner, t->inner_stride)) return fth::fail(FT_EINVAL, "token strides are too large");
     const uint64_t n = t->outer * t->inner;
     if (n && !t->ids) return fth::fail(FT_EINVAL, "ids must not be NULL");
     if (reinterpret_cast<uintptr_t>(t->ids) % static_cast<uintptr_t>(t->id_bytes)) return fth::fail(FT_EALIGN, "ids are not aligned to their size");
