@@ -360,9 +360,11 @@ int ft_synth_fill_host(void* out, int dtype, size_t n, uint64_t seed, uint32_t s
  *
  * Strides are in elements; rows may lie apart, the elements of a row lie together. Pointers need the
  * alignment of their element type. Tables have at most 2^31 - 1 rows of at most 2^24 elements, calls at
- * most 2^31 - 1 tokens, whose ids lie within 2^38 ids per dimension, and no more elements than one launch of 2^32 work-items takes (FT_EINVAL beyond: about
- * 1.4e11 for the lookup and 2.5e11 for the gradient, fewer where rows are short). No call allocates or waits, all may be
- * recorded into a HIP graph.
+ * most 2^31 - 1 tokens, whose ids lie within 2^38 ids per dimension, and no more elements than one launch
+ * of 2^32 work-items takes (FT_EINVAL beyond): below 3.4e10 for the lookup, 6.9e10 where both its types have
+ * 16 bits and it drops out; 2.4e11 for the gradient, 4.8e11 where both its types have 16 bits; fewer where
+ * rows are no multiple of what a wavefront takes of them (256 to 1,024 elements). No call allocates or
+ * waits, all may be recorded into a HIP graph.
  *
  * ft_embedding_lookup: out[i][c] = scale * table[row(i)][c], with drop != NULL then dropped out; one
  * product in fp32 per element (by scale / (1 - p), rounded once), rounded to out's type. */
