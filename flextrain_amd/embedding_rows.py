@@ -102,8 +102,10 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, first_row: 
     if grad_into is not None:
         # Nothing that requires a gradient goes into the lookup, yet its backward pass has to run. The
         # leaf that asks for it is new in every call: one that lived on would tie the graphs of
-        # different calls (an eager one and one that is being recorded) to one stream.
-        weight, anchor = weight.detach(), torch.empty(0, requires_grad=True)
+        # different calls (an eager one and one that is being recorded) to one stream. It is on the
+        # table's GPU: at the end of a backward pass autograd makes the caller's stream wait for the
+        # streams of the leaves, which for this one is the stream that the gradient is added on.
+        weight, anchor = weight.detach(), torch.empty(0, device=weight.device, requires_grad=True)
     mask = (dropout, seed, substream, first_index)
     return _Embedding.apply(weight, anchor, tokens, seed if isinstance(seed, Tensor) else None, scale, first_row, padding_token, mask, dtype,
                             grad_into)

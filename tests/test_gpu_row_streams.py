@@ -1,0 +1,85 @@
+"""The row operators on other streams than the default one. What a stream has to wait for is asked of the stream: while
+another one is kept busy, an event behind the pass must not have been reached."""
+import time
+
+import pytest
+import torch
+
+from flextrain_amd import FlexTrainAdam, embedding
+
+pytestmark = pytest.mark.gpu
+
+ROWS, COLS = 900, 72
+
+
+def _gen(cuda, seed):
+    return torch.Generator(device=cuda).manual_seed(seed)
+
+
+def _whole(cuda, shape, seed=0):
+    """Whole numbers: sums without rounding."""
+    return torch.randint(-8, 9, shape, device=cuda, generator=_gen(cuda, seed)).float()
+
+
+def _ids(cuda, n, seed=0):
+    return torch.randint(0, ROWS, (n,), device=cuda, generator=_gen(cuda, seed))
+
+
+def _keep_busy(cuda, stream):
+    """About a quarter of a second of work on the stream."""
+    with torch.cuda.stream(stream):
+        a = torch.ones((8192, 8192), device=cuda, dtype=torch.bfloat16)
+        b = torch.empty_like(a)
+        for _ in range(300):
+            torch.mm(a, a, out=b)
+
+
+def _waits_for(stream, busy):
+    """Whether what is enqueued on ``stream`` now runs behind what ``busy`` still works on."""
+    event = torch.cuda.Event()
+    event.record(stream)
+    time.sleep(0.02)  # an event on an idle stream is reached by then
+    reached = event.query()
+    assert not busy.query(), "the other stream should have been busy for longer"
+    return not reached
+
+
+@pytest.mark.parametrize("n", [100, 5000])
+def test_backward_pass_is_joined_to_its_caller(cuda, n):
+    """The lookup on a side stream, the backward pass called on the default one: what follows there (the step, which
+    reads and clears the accumulator) waits for the gradient."""
+    weight, acc, tokens, dy = _whole(cuda, (ROWS, COLS)), torch.zeros((ROWS, COLS), device=cuda), _ids(cuda, n), _whole(cuda, (n, COLS), 1)
+    embedding(tokens, weight, grad_into=acc.clone()).backward(dy)  # loads the code
+    side, caller = torch.cuda.Stream(), torch.cuda.current_stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        y = embedding(tokens, weight, grad_into=acc)
+    caller.wait_stream(side)
+    _keep_busy(cuda, side)
+    y.backward(dy)
+    assert _waits_for(caller, side)
+    torch.cuda.synchronize()
+    assert torch.equal(acc, torch.zeros_like(acc).index_add_(0, tokens, dy))
+
+
+def test_step_behind_a_lookup_on_another_stream(cuda):
+    """Forward on a side stream that is late in the backward pass, step on the default one: the same as on one stream."""
+    side = torch.cuda.Stream()
+    tables = []
+    for use in (side, torch.cuda.current_stream()):
+        table = torch.nn.Parameter(_whole(cuda, (ROWS, COLS)).bfloat16())
+        opt = FlexTrainAdam([{"params": [table]}], lr=1e-2, gradacc_dtype=torch.float32)
+        torch.cuda.synchronize()
+        for k in range(2):
+            use.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(use):
+                y = opt.embedding(_ids(cuda, 3000, k), table)
+            torch.cuda.current_stream().wait_stream(use)
+            if use is side:
+                _keep_busy(cuda, side)
+            y.backward(_whole(cuda, (3000, COLS), k + 5).bfloat16())
+            opt.update_states()
+            opt.step()
+        torch.cuda.synchronize()
+        tables.append(table.detach().clone())
+    assert torch.equal(*tables) and not torch.equal(tables[0], _whole(cuda, (ROWS, COLS)).bfloat16())
