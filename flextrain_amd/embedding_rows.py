@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _C
-from .rows import Seed, dropout_record, enqueue, gpu_index, row_stride, token_record, with_even_rows
+from .rows import Seed, dropout_record, enqueue, gpu_index, order_of, row_stride, token_record, with_even_rows
 
 
 def _table(name: str, t: Tensor) -> int:
@@ -129,8 +129,11 @@ class _Embedding(torch.autograd.Function):
         scale, first_row, padding_token, (p, seed, substream, first_index) = ctx.options
         shape, dtype, device = ctx.weight
         into = ctx.grad_into
-        grad = torch.empty(shape, dtype=dtype, device=device) if into is None else into
-        embedding_grad_(grad, tokens, with_even_rows(dy), scale=scale, first_row=first_row, padding_token=padding_token,
-                        accumulate=into is not None, dropout=p, seed=seed if seed_tensor is None else seed_tensor, substream=substream,
-                        first_index=first_index)
-        return (grad if into is None else None,) + (None,) * 9
+        options = dict(scale=scale, first_row=first_row, padding_token=padding_token, dropout=p, seed=seed if seed_tensor is None else seed_tensor,
+                       substream=substream, first_index=first_index)
+        if into is None:
+            grad = embedding_grad_(torch.empty(shape, dtype=dtype, device=device), tokens, with_even_rows(dy), accumulate=False, **options)
+            return (grad,) + (None,) * 9
+        with order_of(into):  # the lookups of one table may be on different streams
+            embedding_grad_(into, tokens, with_even_rows(dy), **options)
+        return (None,) * 10

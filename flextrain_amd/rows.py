@@ -1,6 +1,7 @@
 """What the row operators (embedding, dropout) share: argument checks and the C structs they fill."""
 from __future__ import annotations
 
+import threading
 from typing import Optional, Tuple, Union
 
 import torch
@@ -111,3 +112,65 @@ def token_record(tokens: Tensor, first_row: int, padding: Optional[int]) -> Tupl
     elif not -(1 << 63) < padding < 1 << 63:
         raise ValueError("padding_token must be a 64-bit number")
     return _C.Tokens(tokens.data_ptr(), outer, inner, outer_stride, inner_stride, first_row, padding, size, 0), n
+
+
+class StreamOrder:
+    """``with order:`` around what one pass enqueues on the current stream: passes that change the same memory then run
+    one behind the other, whatever streams they are on. A pass on the stream of the one before it waits for nothing.
+
+    Recorded passes are ordered among those of the same recording; how replays lie to other work is up to the
+    program that replays."""
+
+    def __init__(self, device: torch.device):
+        self._device = device
+        self._lock = threading.Lock()
+        self._now: Optional[torch.cuda.Stream] = None
+        self._last: Optional[torch.cuda.Stream] = None           # of the last pass that was not recorded
+        self._event: Optional[torch.cuda.Event] = None           # behind it, unless that is the default stream
+        self._last_recorded: Optional[torch.cuda.Stream] = None
+
+    def __enter__(self) -> None:
+        self._lock.acquire()
+        try:
+            now = self._now = torch.cuda.current_stream(self._device)
+            if torch.cuda.is_current_stream_capturing():
+                last = self._last_recorded
+                if last is not None and last != now and _is_recorded(last):
+                    now.wait_stream(last)
+            elif self._last is not None and self._last != now:
+                if self._event is None:  # the default stream, which is always there to be asked
+                    now.wait_stream(self._last)
+                else:
+                    now.wait_event(self._event)
+        except BaseException:
+            self._lock.release()
+            raise
+
+    def __exit__(self, *exc) -> None:
+        try:
+            now = self._now
+            if torch.cuda.is_current_stream_capturing():
+                self._last_recorded = now
+            else:
+                # A stream of the program's own may be gone by the next pass: the event is recorded now.
+                if now.cuda_stream == 0:
+                    self._event = None
+                else:
+                    if self._last != now or self._event is None:
+                        self._event = torch.cuda.Event()
+                    self._event.record(now)
+                self._last = now
+        finally:
+            self._lock.release()
+
+
+def _is_recorded(stream: torch.cuda.Stream) -> bool:
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def order_of(t: Tensor) -> StreamOrder:
+    """The order of the passes that add into the memory of ``t``. It lives in that memory's own record and goes with it."""
+    kept = t.untyped_storage().__dict__
+    order = kept.get("_flextrain_order")
+    return kept.setdefault("_flextrain_order", StreamOrder(t.device)) if order is None else order

@@ -83,3 +83,78 @@ def test_step_behind_a_lookup_on_another_stream(cuda):
         torch.cuda.synchronize()
         tables.append(table.detach().clone())
     assert torch.equal(*tables) and not torch.equal(tables[0], _whole(cuda, (ROWS, COLS)).bfloat16())
+
+
+@pytest.mark.parametrize("first", ["default", "side", "other side"])
+@pytest.mark.parametrize("graphs", [1, 2])
+def test_two_streams_add_into_one_accumulator(cuda, first, graphs):
+    """Two lookups of one table, the one whose gradient comes first on a busy stream: the other stream's gradient waits,
+    in one backward pass or two, and again with the streams changed."""
+    weight, acc = _whole(cuda, (ROWS, COLS)), torch.zeros((ROWS, COLS), device=cuda)
+    tokens = [_ids(cuda, n, n) for n in (300, 4000)]
+    dy = [_whole(cuda, (n, COLS), n) for n in (300, 4000)]
+    embedding(tokens[1], weight, grad_into=acc.clone()).backward(dy[1])
+    caller = torch.cuda.current_stream()
+    busy, free = {"default": (caller, torch.cuda.Stream()), "side": (torch.cuda.Stream(), caller), "other side": (torch.cuda.Stream(), torch.cuda.Stream())}[first]
+    third = torch.cuda.Stream()  # the backward pass is called here: the default stream would wait for the side streams, or be busy itself
+    torch.cuda.synchronize()
+    for late, early in ((busy, free), (busy, free), (free, busy)):
+        with torch.cuda.stream(early):
+            y1 = embedding(tokens[1], weight, grad_into=acc[:, :])
+        with torch.cuda.stream(late):  # made last: its gradient comes first
+            y0 = embedding(tokens[0], weight, grad_into=acc)
+        torch.cuda.synchronize()
+        _keep_busy(cuda, late)
+        with torch.cuda.stream(third):
+            if graphs == 1:
+                torch.autograd.backward([y0, y1], dy)
+            else:
+                y0.backward(dy[0])
+                with torch.cuda.stream(torch.cuda.Stream()):  # a caller that waits for nothing
+                    y1.backward(dy[1])
+        assert _waits_for(early, late)
+        torch.cuda.synchronize()
+    want = torch.zeros_like(acc)
+    for t, d in zip(tokens, dy):
+        want.index_add_(0, t, d)
+    assert torch.equal(acc, 3 * want)
+
+
+def test_streams_of_a_recording(cuda):
+    """Two lookups of one table on two streams of one recording, eager passes on other streams between the replays."""
+    weight, acc = _whole(cuda, (ROWS, COLS)), torch.zeros((ROWS, COLS), device=cuda)
+    tokens = [_ids(cuda, n, n) for n in (300, 4000)]
+    dy = [_whole(cuda, (n, COLS), n) for n in (300, 4000)]
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def both():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            y1 = embedding(tokens[1], weight, grad_into=acc)
+        y0 = embedding(tokens[0], weight, grad_into=acc)
+        main.wait_stream(side)
+        torch.autograd.backward([y0, y1], dy)
+
+    want = torch.zeros_like(acc)
+    for t, d in zip(tokens, dy):
+        want.index_add_(0, t, d)
+    graphs = []
+    with torch.cuda.stream(other):
+        both()  # eager, on streams that the recordings do not have
+    torch.cuda.synchronize()
+    assert torch.equal(acc, want)
+    for _ in range(2):  # the second recording has nothing to do with the first one's
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            both()
+    for k in range(3):
+        for graph in graphs:
+            acc.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(acc, want)
+        with torch.cuda.stream(other if k % 2 else torch.cuda.current_stream()):
+            both()
+        torch.cuda.synchronize()
+        assert torch.equal(acc, 2 * want)
