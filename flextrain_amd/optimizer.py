@@ -27,6 +27,7 @@ from .param_group import (
     create_group_segments,
     create_step_contexts,
 )
+from .rows import order_of
 
 STEP_KEY = "step"
 PARAMS_KEY = "params"
@@ -285,9 +286,14 @@ class FlexTrainOptimizer:
 
         def _accumulate_into(i: int):
             def hook(grad: Tensor):
-                acc_views[i] += grad.flatten()
+                if non_layerwise_params[i] in self._embedding_tables:
+                    with order_of(acc_views[i]):
+                        acc_views[i] += grad.flatten()
+                else:
+                    acc_views[i] += grad.flatten()
             return hook
 
+        self._embedding_tables: set = set()
         self._param_offsets: Dict[Tensor, int] = {}
         offset = 0
         for i, param in enumerate(non_layerwise_params):
@@ -343,7 +349,19 @@ class FlexTrainOptimizer:
         through a hook, reference ``flextrain/optimizer.py:194-215``). ``options``: those of
         ``flextrain_amd.embedding`` except ``grad_into``."""
         from .embedding_rows import embedding  # local import: keeps module load light
-        return embedding(tokens, param, grad_into=self.gradient_of(param), **options)
+        into = self.gradient_of(param)
+        if param not in self._embedding_tables:
+            self._order_gradients(param, into)
+        return embedding(tokens, param, grad_into=into, **options)
+
+    def _order_gradients(self, param: Tensor, into: Tensor) -> None:
+        """Gradients of ``param`` that come from elsewhere (a table that is the output layer too) are added on a stream of
+        autograd's choice: they take turns with those of the lookups, which are added on the lookups' streams."""
+        if not self._gradacc_dtype_incompatible:  # autograd adds into param.grad itself; otherwise the accumulating hook does
+            order = order_of(into)
+            param.register_hook(lambda grad: order.wait())
+            param.register_post_accumulate_grad_hook(lambda _: order.mark())
+        self._embedding_tables.add(param)
 
     def step(self, *args, **kwargs):
         """Steps the non-layerwise parameters (reference ``flextrain/optimizer.py:244-263``).

@@ -124,7 +124,6 @@ class StreamOrder:
     def __init__(self, device: torch.device):
         self._device = device
         self._lock = threading.Lock()
-        self._now: Optional[torch.cuda.Stream] = None
         self._last: Optional[torch.cuda.Stream] = None           # of the last pass that was not recorded
         self._event: Optional[torch.cuda.Event] = None           # behind it, unless that is the default stream
         self._last_recorded: Optional[torch.cuda.Stream] = None
@@ -132,36 +131,44 @@ class StreamOrder:
     def __enter__(self) -> None:
         self._lock.acquire()
         try:
-            now = self._now = torch.cuda.current_stream(self._device)
-            if torch.cuda.is_current_stream_capturing():
-                last = self._last_recorded
-                if last is not None and last != now and _is_recorded(last):
-                    now.wait_stream(last)
-            elif self._last is not None and self._last != now:
-                if self._event is None:  # the default stream, which is always there to be asked
-                    now.wait_stream(self._last)
-                else:
-                    now.wait_event(self._event)
+            self.wait()
         except BaseException:
             self._lock.release()
             raise
 
     def __exit__(self, *exc) -> None:
         try:
-            now = self._now
-            if torch.cuda.is_current_stream_capturing():
-                self._last_recorded = now
-            else:
-                # A stream of the program's own may be gone by the next pass: the event is recorded now.
-                if now.cuda_stream == 0:
-                    self._event = None
-                else:
-                    if self._last != now or self._event is None:
-                        self._event = torch.cuda.Event()
-                    self._event.record(now)
-                self._last = now
+            self.mark()
         finally:
             self._lock.release()
+
+    def wait(self) -> None:
+        """The current stream waits for the last pass."""
+        now = torch.cuda.current_stream(self._device)
+        if torch.cuda.is_current_stream_capturing():
+            last = self._last_recorded
+            if last is not None and last != now and _is_recorded(last):
+                now.wait_stream(last)
+        elif self._last is not None and self._last != now:
+            if self._event is None:  # the default stream, which is always there to be asked
+                now.wait_stream(self._last)
+            else:
+                now.wait_event(self._event)
+
+    def mark(self) -> None:
+        """What has been enqueued on the current stream is the last pass."""
+        now = torch.cuda.current_stream(self._device)
+        if torch.cuda.is_current_stream_capturing():
+            self._last_recorded = now
+            return
+        # A stream of the program's own may be gone by the next pass: the event is recorded now.
+        if now.cuda_stream == 0:
+            self._event = None
+        else:
+            if self._last != now or self._event is None:
+                self._event = torch.cuda.Event()
+            self._event.record(now)
+        self._last = now
 
 
 def _is_recorded(stream: torch.cuda.Stream) -> bool:

@@ -158,3 +158,55 @@ def test_streams_of_a_recording(cuda):
             both()
         torch.cuda.synchronize()
         assert torch.equal(acc, 2 * want)
+
+
+@pytest.mark.parametrize("gradacc", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lookup_first", [True, False])
+def test_a_table_with_another_gradient(cuda, gradacc, lookup_first):
+    """A table that is looked up on one stream and used as a matrix on another: the gradient that comes second, in the hook
+    or in autograd's own addition, waits for the first one's busy stream."""
+    table = torch.nn.Parameter(_whole(cuda, (ROWS, COLS)).bfloat16())
+    opt = FlexTrainAdam([{"params": [table]}], lr=1e-2, gradacc_dtype=gradacc)
+    tokens, dy, dz = _ids(cuda, 300), _whole(cuda, (300, COLS), 1).bfloat16().sign(), _whole(cuda, (ROWS, COLS), 2).bfloat16()
+    caller, side, third = torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()
+
+    def lookup():
+        with torch.cuda.stream(side):
+            return opt.embedding(tokens, table)
+
+    opt.embedding(tokens, table).backward(dy)
+    want = torch.zeros((ROWS, COLS), device=cuda).index_add_(0, tokens, dy.float())
+    for k in range(2):
+        torch.cuda.synchronize()
+        if lookup_first:  # made last, its gradient comes first
+            z, y = table * 2.0, lookup()
+            first, second = side, caller
+        else:
+            y, z = lookup(), table * 2.0
+            first, second = caller, side
+        torch.cuda.synchronize()
+        _keep_busy(cuda, first)
+        with torch.cuda.stream(third):
+            torch.autograd.backward([y, z], [dy, dz])
+        assert _waits_for(second, first)
+        torch.cuda.synchronize()
+    want = 3 * want + 4.0 * dz.float()  # whole numbers; in 16 bits below 256: exact
+    assert float(want.abs().max()) < 256 and torch.equal(opt.gradient_of(table).float(), want)
+    assert len(torch.autograd.grad(table.sum(), table)) == 1 and opt.gradient_of(table).any()
+
+
+def test_a_table_with_another_gradient_on_one_stream(cuda):
+    """Lookup and output layer share the table, as models with tied weights do."""
+    for gradacc in (torch.float32, torch.bfloat16):
+        table = torch.nn.Parameter(_whole(cuda, (ROWS, COLS)).bfloat16())
+        opt = FlexTrainAdam([{"params": [table]}], lr=1e-2, gradacc_dtype=gradacc)
+        tokens, weights = _ids(cuda, 40), _whole(cuda, (40, ROWS), 3).bfloat16().sign()
+        x = opt.embedding(tokens, table)
+        (x @ table.t()).backward(weights)
+        direct = weights.float().t() @ table.detach().float()[tokens]
+        rows = weights.float() @ table.detach().float()
+        want = direct.double().index_add_(0, tokens, rows.double())
+        got = opt.gradient_of(table).double()
+        # both gradients arrive rounded to bf16, their sum is rounded to the accumulator's type; tokens met twice add up rounded rows
+        terms = direct.abs().double().index_add_(0, tokens, rows.abs().double())
+        assert bool(((got - want).abs() <= 2.1 * 2.0 ** -8 * terms).all())
