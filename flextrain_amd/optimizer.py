@@ -347,9 +347,12 @@ class FlexTrainOptimizer:
         gradient straight into the buffer the step reads, only in the rows that a token names. Without
         it, every micro-batch makes a dense gradient of the whole table and adds that (in a wider type
         through a hook, reference ``flextrain/optimizer.py:194-215``). ``options``: those of
-        ``flextrain_amd.embedding`` except ``grad_into``."""
+        ``flextrain_amd.embedding`` except ``grad_into``. A frozen table (``requires_grad``
+        False) has no gradient, as with torch's."""
         from .embedding_rows import embedding  # local import: keeps module load light
         into = self.gradient_of(param)
+        if not param.requires_grad:  # a frozen table
+            return embedding(tokens, param, **options)
         if param not in self._embedding_tables:
             self._order_gradients(param, into)
         return embedding(tokens, param, grad_into=into, **options)
