@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 
 from . import _C
-from .rows import Seed, dropout_record, enqueue, gpu_index, row_stride, with_even_rows
+from .rows import Seed, dropout_record, enqueue, gpu_index, row_stride, with_even_rows, written
 
 
 def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index: int = 0, residual: Optional[Tensor] = None,
@@ -44,6 +44,7 @@ def _apply(x: Tensor, p: float, seed: Seed, substream: int, first_index: int, re
     if dtype is None:
         dtype = x.dtype if residual is None else residual.dtype
     cols = shape[-1] if shape else 1
+    given = out
     if out is None:
         out, out_stride = x.new_empty(shape, dtype=dtype), cols
     elif out.shape != shape or out.dtype != dtype:
@@ -56,7 +57,7 @@ def _apply(x: Tensor, p: float, seed: Seed, substream: int, first_index: int, re
             None if residual is None else residual.data_ptr(), 0 if residual is None else row_stride("residual", residual, cols),
             out.data_ptr(), _C.dtype_code(dtype), out_stride, rows, cols,
             ctypes.byref(dropout_record(index, p, seed, substream, first_index)))
-    return out
+    return out if given is None else written(out)
 
 
 class _Dropout(torch.autograd.Function):

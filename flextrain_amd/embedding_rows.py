@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _C
-from .rows import Seed, dropout_record, enqueue, gpu_index, order_of, row_stride, token_record, with_even_rows
+from .rows import Seed, dropout_record, enqueue, gpu_index, order_of, row_stride, token_record, with_even_rows, written
 
 
 def _table(name: str, t: Tensor) -> int:
@@ -41,6 +41,7 @@ def embedding_lookup(tokens: Tensor, table: Tensor, *, scale: float = 1.0, first
     table_stride = _table("table", table)
     rows, cols = table.shape
     shape = (*tokens.shape, cols)
+    given = out
     if out is None:
         out, out_stride = table.new_empty(shape, dtype=dtype), cols
     elif out.shape != shape or (dtype is not None and out.dtype != dtype):
@@ -52,7 +53,7 @@ def embedding_lookup(tokens: Tensor, table: Tensor, *, scale: float = 1.0, first
             ctypes.byref(record), table.data_ptr(), _C.dtype_code(table.dtype), rows, table_stride, out.data_ptr(), _C.dtype_code(out.dtype),
             out_stride, cols, scale,
             None if dropout == 0.0 else ctypes.byref(dropout_record(index, dropout, seed, substream, first_index)))
-    return out
+    return out if given is None else written(out)
 
 
 def embedding_grad_(acc: Tensor, tokens: Tensor, grads: Tensor, *, scale: float = 1.0, first_row: int = 0, padding_token: Optional[int] = None,
@@ -78,7 +79,7 @@ def embedding_grad_(acc: Tensor, tokens: Tensor, grads: Tensor, *, scale: float 
             _C.dtype_code(acc.dtype), rows, acc_stride, cols, scale, int(bool(accumulate)),
             None if dropout == 0.0 else ctypes.byref(dropout_record(index, dropout, seed, substream, first_index)),
             None if workspace is None else workspace.data_ptr(), need)
-    return acc
+    return written(acc)
 
 
 def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, first_row: int = 0, padding_token: Optional[int] = None,

@@ -13,7 +13,6 @@ from . import _C
 Seed = Union[int, Tensor]
 
 
-
 def gpu_index(**tensors: Optional[Tensor]) -> int:
     """The GPU that all of the tensors (those that are not None) are on."""
     index = None
@@ -38,6 +37,13 @@ def enqueue(name: str, fn, index: int, *args) -> None:
             rc = fn(*args, _C.current_stream_ptr(index))
     if rc:
         _C.check(name, rc)
+
+
+def written(t: Tensor) -> Tensor:
+    """Tells autograd that a kernel has written into ``t``: a backward pass that needs its old values then raises."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+    return t
 
 
 def row_stride(name: str, t: Tensor, cols: int) -> int:

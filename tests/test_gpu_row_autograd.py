@@ -32,3 +32,44 @@ def test_a_frozen_table_has_no_gradient(cuda, gradacc, used_before):
     table.requires_grad_(True)
     opt.embedding(tokens, table).backward(dy)
     assert torch.equal(opt.gradient_of(table)[:30], before[:30] + 1) and torch.equal(opt.gradient_of(table)[30:], before[30:])
+
+
+WRITES = {
+    "dropout": lambda t: dropout(torch.ones_like(t), 0.1, 1, out=t),
+    "dropout in place": lambda t: dropout(t, 0.1, 1, out=t),
+    "dropout onto the residual": lambda t: dropout(torch.ones_like(t), 0.1, 1, residual=t, out=t),
+    "lookup": lambda t: embedding_lookup(torch.arange(t.shape[0], device=t.device), torch.ones_like(t), out=t),
+    "gradient": lambda t: embedding_grad_(t, torch.arange(t.shape[0], device=t.device), torch.ones_like(t)),
+}
+
+
+@pytest.mark.parametrize("write", WRITES)
+@pytest.mark.parametrize("through_a_view", [False, True])
+def test_writes_into_given_tensors_are_found_out(cuda, write, through_a_view):
+    """As with torch's own operators: a backward pass that needs the old values of a tensor that was written raises."""
+    x, w = _randn(cuda, (20, 12), F32), _randn(cuda, (20, 12), F32, 1).requires_grad_()
+    h = x * w  # w's gradient needs x
+    before = x._version
+    with torch.no_grad():
+        WRITES[write](x[3:9] if through_a_view else x)
+    assert x._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+
+
+def test_a_gradient_added_by_a_backward_pass_is_found_out(cuda):
+    weight, acc = _randn(cuda, (20, 12), F32), _randn(cuda, (20, 12), F32, 1)
+    w = _randn(cuda, (20, 12), F32, 2).requires_grad_()
+    h = acc * w
+    embedding(torch.arange(9, device=cuda), weight, grad_into=acc).sum().backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+
+
+@pytest.mark.parametrize("write", WRITES)
+def test_writes_without_autograd(cuda, write):
+    x = _randn(cuda, (20, 12), F32)
+    want = WRITES[write](x.clone())
+    with torch.inference_mode():
+        inside = x.clone()
+        assert inside.is_inference() and torch.equal(WRITES[write](inside), want)
