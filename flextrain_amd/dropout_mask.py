@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 
 from . import _C
-from .rows import Seed, dropout_record, enqueue, gpu_index, row_stride, with_even_rows, written
+from .rows import Seed, dropout_record, enqueue, gpu_index, refuse_leaves, row_stride, with_even_rows, written
 
 
 def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index: int = 0, residual: Optional[Tensor] = None,
@@ -30,8 +30,8 @@ def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index:
     """
     if out is None and torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, residual, float(p), seed, substream, first_index, seed if isinstance(seed, Tensor) else None)
-    if out is not None and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, out)):
-        raise ValueError("out: not for tensors that require gradients")
+    if out is not None:
+        refuse_leaves("out", x, residual, out)
     return _apply(x, float(p), seed, substream, first_index, residual, out)
 
 

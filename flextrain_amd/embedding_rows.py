@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _C
-from .rows import Seed, dropout_record, enqueue, gpu_index, order_of, row_stride, token_record, with_even_rows, written
+from .rows import Seed, dropout_record, enqueue, gpu_index, order_of, refuse_leaves, row_stride, token_record, with_even_rows, written
 
 
 def _table(name: str, t: Tensor) -> int:
@@ -42,6 +42,8 @@ def embedding_lookup(tokens: Tensor, table: Tensor, *, scale: float = 1.0, first
     rows, cols = table.shape
     shape = (*tokens.shape, cols)
     given = out
+    if out is not None and out.requires_grad:
+        refuse_leaves("out", out)
     if out is None:
         out, out_stride = table.new_empty(shape, dtype=dtype), cols
     elif out.shape != shape or (dtype is not None and out.dtype != dtype):
@@ -66,6 +68,8 @@ def embedding_grad_(acc: Tensor, tokens: Tensor, grads: Tensor, *, scale: float 
     applied to ``grads`` first. Sums are kept in fp32 and rounded to acc's type once; the same call
     gives the same bits."""
     index = gpu_index(acc=acc, tokens=tokens, grads=grads)
+    if acc.requires_grad:
+        refuse_leaves("acc", acc)
     acc_stride = _table("acc", acc)
     rows, cols = acc.shape
     if grads.shape != (*tokens.shape, cols):

@@ -46,6 +46,12 @@ def written(t: Tensor) -> Tensor:
     return t
 
 
+def refuse_leaves(name: str, *tensors: Optional[Tensor]) -> None:
+    """What is written outside autograd must not be part of a graph."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name}: not for tensors that require gradients")
+
+
 def row_stride(name: str, t: Tensor, cols: int) -> int:
     """Distance of the rows of ``t`` (its last dimension) in elements: the elements of a row must lie
     together and the rows at one common distance."""

@@ -73,3 +73,17 @@ def test_writes_without_autograd(cuda, write):
     with torch.inference_mode():
         inside = x.clone()
         assert inside.is_inference() and torch.equal(WRITES[write](inside), want)
+
+
+def test_results_given_by_the_caller_must_not_require_gradients(cuda):
+    leaf, ids = _randn(cuda, (5, 8), F32).requires_grad_(), torch.arange(5, device=cuda)
+    kept = leaf.detach().clone()
+    for call in (lambda: embedding_lookup(ids, kept, out=leaf), lambda: embedding_grad_(leaf, ids, kept),
+                 lambda: embedding_lookup(ids, kept, out=leaf * 1.0)):
+        with pytest.raises(ValueError, match="require gradients"):
+            call()
+    assert torch.equal(leaf, kept)
+    with torch.no_grad():  # as an update of one's own
+        embedding_grad_(leaf, ids, kept, scale=-1.0)
+        assert not bool(leaf.any())
+        assert torch.equal(embedding_lookup(ids, kept, out=leaf), kept)
