@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _C
-from .rows import Seed, dropout_record, enqueue, gpu_index, order_of, refuse_leaves, row_stride, token_record, with_even_rows, written
+from .rows import Seed, dropout_record, enqueue, gpu_index, order_of, refuse_leaves, refuse_tangents, row_stride, token_record, with_even_rows, written
 
 
 def _table(name: str, t: Tensor) -> int:
@@ -94,6 +94,7 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, first_row: 
     gradient there, row by row. Hooks of ``weight`` do not run in that case.
 
     A ``seed`` in GPU memory, and the tokens, must keep their values until the backward pass has run."""
+    refuse_tangents(weight=weight)  # detach() below would drop it
     if grad_into is not None:
         gpu_index(weight=weight, grad_into=grad_into)
         if grad_into.shape != weight.shape:

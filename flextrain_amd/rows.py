@@ -6,6 +6,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _C
 
@@ -15,6 +16,8 @@ Seed = Union[int, Tensor]
 
 def gpu_index(**tensors: Optional[Tensor]) -> int:
     """The GPU that all of the tensors (those that are not None) are on."""
+    if forward_ad._current_level >= 0:
+        refuse_tangents(**tensors)
     index = None
     for name, t in tensors.items():
         if t is None:
@@ -25,6 +28,13 @@ def gpu_index(**tensors: Optional[Tensor]) -> int:
         if at < 0 or at != index:
             raise ValueError(f"{name} must be a tensor on the GPU" + (f" {index}" if index >= 0 and at >= 0 else ""))
     return index
+
+
+def refuse_tangents(**tensors: Optional[Tensor]) -> None:
+    """The operators have no forward-mode derivative: the kernels see no tangent, and the result would have none."""
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has a forward-mode derivative, which this operator does not carry on")
 
 
 def enqueue(name: str, fn, index: int, *args) -> None:

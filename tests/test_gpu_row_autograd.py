@@ -87,3 +87,22 @@ def test_results_given_by_the_caller_must_not_require_gradients(cuda):
         embedding_grad_(leaf, ids, kept, scale=-1.0)
         assert not bool(leaf.any())
         assert torch.equal(embedding_lookup(ids, kept, out=leaf), kept)
+
+
+@pytest.mark.parametrize("needs", [False, True])
+def test_forward_mode_is_refused(cuda, needs):
+    """A tangent must not vanish without a word."""
+    x, ids = _randn(cuda, (6, 8), F32).requires_grad_(needs), torch.arange(6, device=cuda)
+    plain = x.detach().clone()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(plain))
+        for call in (lambda: dropout(dual, 0.1, 1), lambda: dropout(plain, 0.1, 1, residual=dual), lambda: embedding_lookup(ids, dual),
+                     lambda: embedding(ids, dual), lambda: embedding(ids, dual, grad_into=plain.clone()),
+                     lambda: embedding_grad_(plain.clone(), ids, dual)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(embedding_lookup(ids, plain), plain)  # without a tangent, as ever
+        assert torch.equal(dropout(plain, 0.0, 1), plain)
+        assert torch.equal(embedding_grad_(torch.zeros_like(plain), ids, plain), plain)
+    with torch.no_grad():
+        assert torch.equal(embedding(ids, x), plain)
