@@ -20,7 +20,7 @@ from .rows import Seed, dropout_record, enqueue, gpu_index, refuse_leaves, row_s
 
 def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index: int = 0, residual: Optional[Tensor] = None,
             out: Optional[Tensor] = None) -> Tensor:
-    """``[residual +] keep * x / (1 - p)``, differentiable in ``x`` and ``residual``.
+    """``[residual +] keep * x / (1 - p)``, differentiable in ``x`` and ``residual``, any number of times.
 
     ``x``: fp32 / fp16 / bf16 GPU tensor whose rows (last dimension) lie at one distance. ``residual``
     has x's shape; its type is the result's (without one, x's is). ``seed``: a number, or one int64
@@ -29,7 +29,7 @@ def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index:
     ``x`` or ``residual``. A dropped element contributes 0 even where ``x`` is inf or nan.
     """
     if out is None and torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, float(p), seed, substream, first_index, seed if isinstance(seed, Tensor) else None)
+        return _Dropout.apply(x, residual, float(p), seed, substream, first_index, seed if isinstance(seed, Tensor) else None, None)
     if out is not None:
         refuse_leaves("out", x, residual, out)
     return _apply(x, float(p), seed, substream, first_index, residual, out)
@@ -62,18 +62,21 @@ def _apply(x: Tensor, p: float, seed: Seed, substream: int, first_index: int, re
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, substream, first_index, seed_tensor):
+    def forward(ctx, x, residual, p, seed, substream, first_index, seed_tensor, dtype):
         ctx.save_for_backward(seed_tensor)  # a seed that changes before the backward pass is found out
         ctx.mask = (p, seed, substream, first_index)
         ctx.x_dtype = x.dtype
-        return _apply(x, p, seed, substream, first_index, residual)
+        return _apply(x, p, seed, substream, first_index, residual, dtype=dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         (seed_tensor,) = ctx.saved_tensors
         p, seed, substream, first_index = ctx.mask
         dx = None
         if ctx.needs_input_grad[0]:
-            dx = _apply(with_even_rows(dy), p, seed if seed_tensor is None else seed_tensor, substream, first_index, dtype=ctx.x_dtype)
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
+            g = with_even_rows(dy)
+            if torch.is_grad_enabled() and g.requires_grad:  # linear: the gradient of the gradient is the operator again
+                dx = _Dropout.apply(g, None, p, seed, substream, first_index, seed_tensor, ctx.x_dtype)
+            else:
+                dx = _apply(g, p, seed if seed_tensor is None else seed_tensor, substream, first_index, dtype=ctx.x_dtype)
+        return (dx, dy if ctx.needs_input_grad[1] else None) + (None,) * 6

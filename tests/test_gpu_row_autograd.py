@@ -106,3 +106,44 @@ def test_forward_mode_is_refused(cuda, needs):
         assert torch.equal(embedding_grad_(torch.zeros_like(plain), ids, plain), plain)
     with torch.no_grad():
         assert torch.equal(embedding(ids, x), plain)
+
+
+@pytest.mark.parametrize("dtype,residual_dtype", [(F32, None), (F32, F32), (BF16, F32), (F32, BF16), (F16, None)])
+@pytest.mark.parametrize("seed_in_memory", [False, True])
+def test_dropout_twice_differentiated(cuda, dtype, residual_dtype, seed_in_memory):
+    """The operator is linear: its backward pass is the operator again, and so on."""
+    p, shape = 0.25, (33, 40)
+    seed = torch.tensor([9], dtype=torch.int64, device=cuda) if seed_in_memory else 9
+    x = _randn(cuda, shape, dtype).requires_grad_()
+    residual = None if residual_dtype is None else _randn(cuda, shape, residual_dtype, 1).requires_grad_()
+    leaves = [x] if residual is None else [x, residual]
+    factor = ref.kept(shape, p, 9, 3).to(cuda) / (1.0 - p)  # 4 / 3: each product is rounded to fp32, then to its type
+
+    y = dropout(x, p, seed, substream=3, residual=residual)
+    first = torch.autograd.grad((y * y).sum() / 2, leaves, create_graph=True)  # y * factor, and y
+    assert all(g.requires_grad for g in first)
+    u = [torch.ones_like(g) * 2.0 for g in first]
+    second = torch.autograd.grad(first, leaves, u)
+    # first = J' y, y = J leaves: second = J' J u with J = [diag(factor), 1]
+    ju = 2.0 * factor + (0.0 if residual is None else 2.0)
+    wants = [factor * ju] + ([] if residual is None else [ju])
+    for got, want in zip(second, wants):
+        # five values are rounded one behind the other, to fp32 and to the coarsest of the types
+        coarse = max(ref.HALF_STEP[t] for t in (dtype, residual_dtype) if t is not None)
+        assert bool(((got.double() - want).abs() <= 5 * 1.01 * (coarse + ref.F32) * want.abs()).all())
+
+
+def test_gradient_of_a_gradient_penalty(cuda):
+    """A gradient with respect to the gradient that came in, as a penalty on gradients needs it."""
+    x, w = _randn(cuda, (20, 24), F32).requires_grad_(), _randn(cuda, (20, 24), F32, 1).requires_grad_()
+    keep = ref.kept((20, 24), 0.5, 4).to(cuda).float() * 2.0  # exact in fp32
+    g, = torch.autograd.grad((dropout(x, 0.5, 4) * w).sum(), x, create_graph=True)
+    want, = torch.autograd.grad((x * keep * w).sum(), x, create_graph=True)
+    assert torch.equal(g, want)
+    got_w, = torch.autograd.grad(g.pow(2).sum(), w)
+    want_w, = torch.autograd.grad(want.pow(2).sum(), w)
+    assert torch.equal(got_w, want_w)
+    # a transposed gradient of the gradient
+    g, = torch.autograd.grad((dropout(x, 0.5, 4).t() * w.t()).sum(), x, create_graph=True)
+    got_w, = torch.autograd.grad(g.t().pow(2).sum(), w)
+    assert torch.equal(got_w, want_w)
