@@ -155,6 +155,10 @@ int ft_dropout(const void* x, int x_dtype, size_t x_stride, const void* residual
     if (rows > 1 && out_stride < cols) return fth::fail(FT_EINVAL, "rows of out overlap: stride %zu, %zu elements", out_stride, cols);
     if (!ftr::aligned_to(x, x_dtype) || !ftr::aligned_to(out, out_dtype) || !ftr::aligned_to(residual, out_dtype))
         return fth::fail(FT_EALIGN, "x, residual and out must be aligned to their element size");
+    const ftr::Rows from{x, x_dtype, rows, x_stride, cols}, added{residual, out_dtype, residual ? rows : 0, residual_stride, cols},
+        to{out, out_dtype, rows, out_stride, cols};
+    if ((!ftr::same_rows(from, to) && ftr::overlap(from, to)) || (!ftr::same_rows(added, to) && ftr::overlap(added, to)))
+        return fth::fail(FT_EINVAL, "out overlaps x or residual and is not the same array");
     a.x = x;
     a.residual = residual;
     a.out = out;

@@ -1322,6 +1322,8 @@ int ft_embedding_lookup(const ft_tokens_t* tokens, const void* table, int table_
         a.factor = a.drop.factor;
     }
     if (a.tokens.n == 0 || cols == 0) return FT_OK;
+    if (ftr::overlap({table, table_dtype, rows, table_stride, cols}, {out, out_dtype, a.tokens.n, out_stride, cols}))
+        return fth::fail(FT_EINVAL, "out overlaps the table");
     a.tokens.padding = FT_NO_PADDING;  // padding has a row like any other token
     a.table = table;
     a.out = out;
@@ -1371,6 +1373,8 @@ int ft_embedding_grad(const ft_tokens_t* tokens, const void* g, int g_dtype, siz
     // the sums' launch holds at most 2^32 - 1 work-items
     if (static_cast<uint64_t>(plan.groups) * (plan.padded / (kLanes * unit)) + kMostClearing > 0xffffffffull / (kSumWaves * kLanes))
         return fth::fail(FT_EINVAL, "%u tokens of %zu elements are too many for one call", a.tokens.n, cols);
+    if (ftr::overlap({g, g_dtype, a.tokens.n, g_stride, cols}, {acc, acc_dtype, rows, acc_stride, cols}))
+        return fth::fail(FT_EINVAL, "acc overlaps the gradient rows");
     a.g = g;
     a.acc = acc;
     a.g_stride = g_stride;

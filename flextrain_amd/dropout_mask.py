@@ -26,7 +26,7 @@ def dropout(x: Tensor, p: float, seed: Seed, *, substream: int = 0, first_index:
     has x's shape; its type is the result's (without one, x's is). ``seed``: a number, or one int64
     element of GPU memory -- then a pass recorded into a HIP graph follows a seed that changes between
     replays; it must keep its value until the backward pass has run. ``out`` (no gradients then) may be
-    ``x`` or ``residual``. A dropped element contributes 0 even where ``x`` is inf or nan.
+    ``x`` or ``residual``, or memory of its own. A dropped element contributes 0 even where ``x`` is inf or nan.
     """
     if out is None and torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, residual, float(p), seed, substream, first_index, seed if isinstance(seed, Tensor) else None, None)

@@ -367,7 +367,8 @@ int ft_synth_fill_host(void* out, int dtype, size_t n, uint64_t seed, uint32_t s
  * waits, all may be recorded into a HIP graph.
  *
  * ft_embedding_lookup: out[i][c] = scale * table[row(i)][c], with drop != NULL then dropped out; one
- * product in fp32 per element (by scale / (1 - p), rounded once), rounded to out's type. */
+ * product in fp32 per element (by scale / (1 - p), rounded once), rounded to out's type. out shares no memory
+ * with the table, acc below none with g (FT_EINVAL). */
 #define FT_NO_PADDING INT64_MIN
 typedef struct ft_tokens_t {
     const void* ids;
@@ -404,8 +405,8 @@ int ft_embedding_grad(const ft_tokens_t* tokens, const void* g, int g_dtype, siz
 /* ---- dropout -----------------------------------------------------------------------------------
  * out = [residual +] dropout(x) for rows x cols elements (see ft_dropout_t above); the product is rounded to fp32,
  * the sum to fp32 and to out's type. residual (NULL: none)
- * has out's type; out may be x or residual itself where type and strides agree. A dropped element
- * contributes 0, whatever x holds there. The gradient of x is the same call on the gradient of out,
+ * has out's type; out may be x or residual itself where type and strides agree, and shares no memory with
+ * them otherwise (FT_EINVAL). A dropped element contributes 0, whatever x holds there. The gradient of x is the same call on the gradient of out,
  * without residual; that of residual is the gradient of out. No counterpart in the reference, whose
  * models drop out through torch with a stored mask. */
 int ft_dropout(const void* x, int x_dtype, size_t x_stride, const void* residual, size_t residual_stride, void* out, int out_dtype,

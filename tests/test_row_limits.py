@@ -9,6 +9,7 @@ from flextrain_amd import _C
 F32, F16, BF16 = _C.F32, _C.F16, _C.BF16
 BUF = (ctypes.c_double * 64)()
 ADDR = (ctypes.addressof(BUF) + 15) // 16 * 16
+FAR = 1 << 60  # nothing is read or written
 EINVAL = -1
 
 
@@ -26,7 +27,7 @@ def _refused(rc):
 def test_elements_of_a_lookup(table_dtype, out_dtype, p, limit, cols):
     """2^35 is 3.4e10."""
     drop = ctypes.byref(_C.Dropout(p, 1, None, 0, 0, 0))
-    _refused(_C.lib().ft_embedding_lookup(_tokens(limit // cols), ADDR, table_dtype, 4, cols, ADDR, out_dtype, cols, cols, 1.0, drop, None))
+    _refused(_C.lib().ft_embedding_lookup(_tokens(limit // cols), ADDR, table_dtype, 4, cols, FAR, out_dtype, cols, cols, 1.0, drop, None))
 
 
 @pytest.mark.parametrize("g_dtype,acc_dtype,limit", [(BF16, F32, 2.41e11), (F32, F16, 2.41e11), (F16, BF16, 4.82e11)])
