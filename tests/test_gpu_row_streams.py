@@ -5,7 +5,7 @@ import time
 import pytest
 import torch
 
-from flextrain_amd import FlexTrainAdam, embedding
+from flextrain_amd import FlexTrainAdam, dropout, embedding, embedding_grad_, embedding_lookup
 
 pytestmark = pytest.mark.gpu
 
@@ -210,3 +210,38 @@ def test_a_table_with_another_gradient_on_one_stream(cuda):
         # both gradients arrive rounded to bf16, their sum is rounded to the accumulator's type; tokens met twice add up rounded rows
         terms = direct.abs().double().index_add_(0, tokens, rows.abs().double())
         assert bool(((got - want).abs() <= 2.1 * 2.0 ** -8 * terms).all())
+
+
+@pytest.mark.parametrize("call", ["dropout", "lookup", "gradient of few", "gradient of many", "gradient written", "embedding"])
+def test_calls_run_on_the_current_stream(cuda, call):
+    """Inputs that are ready late on a side stream, results that are read there: a kernel on another stream would take the
+    old inputs, or come too late."""
+    n = 100 if call == "gradient of few" else 20000
+    new = dict(x=_whole(cuda, (n, COLS), 1), table=_whole(cuda, (ROWS, COLS), 2), tokens=_ids(cuda, n, 3), acc=_whole(cuda, (ROWS, COLS), 4))
+    old = {k: torch.zeros_like(v) for k, v in new.items()}
+
+    def run(x, table, tokens, acc):
+        if call == "dropout":
+            return dropout(x, 0.1, 3, residual=x)
+        if call == "lookup":
+            return embedding_lookup(tokens, table, dropout=0.1, seed=2)
+        if call == "embedding":
+            weight = table.detach().requires_grad_()
+            y = embedding(tokens, weight, grad_into=acc)
+            y.backward(x)
+            return torch.cat([y.detach(), acc])
+        return embedding_grad_(acc, tokens, x, accumulate=call != "gradient written")
+
+    want = run(**{k: v.clone() for k, v in new.items()})
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    _keep_busy(cuda, side)
+    with torch.cuda.stream(side):
+        for k in new:
+            old[k].copy_(new[k])
+        got = run(**old).clone()
+        assert not side.query(), "the stream should have been busy for longer"
+        for v in old.values():
+            v.zero_()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
