@@ -138,16 +138,16 @@ def token_record(tokens: Tensor, first_row: int, padding: Optional[int]) -> Tupl
 
 class StreamOrder:
     """``with order:`` around what one pass enqueues on the current stream: passes that change the same memory then run
-    one behind the other, whatever streams they are on. A pass on the stream of the one before it waits for nothing.
+    one behind the other, whatever streams they are on. On the default stream alone there is nothing to do.
 
     Recorded passes are ordered among those of the same recording; how replays lie to other work is up to the
     program that replays."""
 
-    def __init__(self, device: torch.device):
-        self._device = device
+    def __init__(self, index: int):
+        self._index = index
         self._lock = threading.Lock()
-        self._last: Optional[torch.cuda.Stream] = None           # of the last pass that was not recorded
-        self._event: Optional[torch.cuda.Event] = None           # behind it, unless that is the default stream
+        self._on_default = False                        # the last pass that was not recorded: on the default stream,
+        self._event: Optional[torch.cuda.Event] = None  # or with this event behind it on another one
         self._last_recorded: Optional[torch.cuda.Stream] = None
 
     def __enter__(self) -> None:
@@ -166,31 +166,30 @@ class StreamOrder:
 
     def wait(self) -> None:
         """The current stream waits for the last pass."""
-        now = torch.cuda.current_stream(self._device)
+        if self._event is None and _C.current_stream_ptr(self._index) == 0:
+            return  # the default stream behind itself
+        now = torch.cuda.current_stream(self._index)
         if torch.cuda.is_current_stream_capturing():
             last = self._last_recorded
             if last is not None and last != now and _is_recorded(last):
                 now.wait_stream(last)
-        elif self._last is not None and self._last != now:
-            if self._event is None:  # the default stream, which is always there to be asked
-                now.wait_stream(self._last)
-            else:
-                now.wait_event(self._event)
+        elif self._event is not None:
+            now.wait_event(self._event)
+        elif self._on_default:
+            now.wait_stream(torch.cuda.default_stream(self._index))
 
     def mark(self) -> None:
         """What has been enqueued on the current stream is the last pass."""
-        now = torch.cuda.current_stream(self._device)
+        if _C.current_stream_ptr(self._index) == 0:  # always there to be waited for, and never recorded
+            self._event, self._on_default = None, True
+            return
+        now = torch.cuda.current_stream(self._index)
         if torch.cuda.is_current_stream_capturing():
             self._last_recorded = now
             return
-        # A stream of the program's own may be gone by the next pass: the event is recorded now.
-        if now.cuda_stream == 0:
-            self._event = None
-        else:
-            if self._last != now or self._event is None:
-                self._event = torch.cuda.Event()
-            self._event.record(now)
-        self._last = now
+        if self._event is None:
+            self._event = torch.cuda.Event()
+        self._event.record(now)  # now: a stream of the program's own may be gone by the next pass
 
 
 def _is_recorded(stream: torch.cuda.Stream) -> bool:
@@ -202,4 +201,4 @@ def order_of(t: Tensor) -> StreamOrder:
     """The order of the passes that add into the memory of ``t``. It lives in that memory's own record and goes with it."""
     kept = t.untyped_storage().__dict__
     order = kept.get("_flextrain_order")
-    return kept.setdefault("_flextrain_order", StreamOrder(t.device)) if order is None else order
+    return kept.setdefault("_flextrain_order", StreamOrder(t.get_device())) if order is None else order
