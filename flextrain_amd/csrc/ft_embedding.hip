@@ -270,9 +270,10 @@ __device__ __forceinline__ RowBits<AT, U> load_old(const GradPass& a, uint32_t r
 // Up to 16,384 tokens: one launch, no workgroup waits for another. Workgroup b looks through ALL
 // tokens (sixteen per thread at most), keeps those whose row ends in the byte b, counts those that go
 // in front of them, and sorts its own by the row's other bits in LDS. That is 256 times the reading, all of it
-// from the L2, and takes 7.5 us where sorting in one workgroup took 23 us (8,192 tokens as text has them), 11 us
-// where the radix sort below took 50 (16,384). What bounds it is the looking through: 60 instructions per token and
-// wavefront.
+// from the L2, and still faster than sorting in one workgroup (23 us for 8,192 tokens as text has them) and than the radix
+// sort below (50 us for 16,384). Uniform tokens take 5.6 us for 8,192 and 8.1 us for 16,384, tokens as text has them 7.7 and
+// 10.9: looking through costs 2.5 us per 8,192 tokens (60 instructions per token and wavefront), the bucket of the most
+// frequent token, which ends the launch, 2 to 3 us, and the launch and the latency of its steps the other 3 us.
 // More: radix sort by digits of at most nine bits, two launches a pass (count 4 us, place 8 us: 131,072 tokens),
 // which are little more than the latency of their steps.
 //
