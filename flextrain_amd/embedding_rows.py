@@ -91,7 +91,8 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, first_row: 
               grad_into: Optional[Tensor] = None) -> Tensor:
     """``embedding_lookup`` for autograd. ``weight`` gets a dense gradient of its own type -- or, with
     ``grad_into`` (shape of ``weight``, fp32 / fp16 / bf16), none: the backward pass then adds the
-    gradient there, row by row. Hooks of ``weight`` do not run in that case.
+    gradient there, row by row, behind whatever else adds into that memory. Hooks of ``weight`` do not
+    run in that case, and a backward pass confined to some leaves (``inputs=``) does not get there.
 
     A ``seed`` in GPU memory, and the tokens, must keep their values until the backward pass has run."""
     refuse_tangents(weight=weight)  # detach() below would drop it

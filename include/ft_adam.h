@@ -403,12 +403,12 @@ int ft_embedding_grad(const ft_tokens_t* tokens, const void* g, int g_dtype, siz
                       size_t workspace_bytes, void* stream);
 
 /* ---- dropout -----------------------------------------------------------------------------------
- * out = [residual +] dropout(x) for rows x cols elements (see ft_dropout_t above); the product is rounded to fp32,
- * the sum to fp32 and to out's type. residual (NULL: none)
- * has out's type; out may be x or residual itself where type and strides agree, and shares no memory with
- * them otherwise (FT_EINVAL). A dropped element contributes 0, whatever x holds there. The gradient of x is the same call on the gradient of out,
- * without residual; that of residual is the gradient of out. No counterpart in the reference, whose
- * models drop out through torch with a stored mask. */
+ * out = [residual +] dropout(x) for rows x cols elements (see ft_dropout_t above); the product is rounded
+ * to fp32, the sum to fp32 and to out's type. residual (NULL: none) has out's type; out may be x or
+ * residual itself where type and strides agree, and shares no memory with them otherwise (FT_EINVAL). A
+ * dropped element contributes 0, whatever x holds there. The gradient of x is the same call on the
+ * gradient of out, without residual; that of residual is the gradient of out. No counterpart in the
+ * reference, whose models drop out through torch with a stored mask. */
 int ft_dropout(const void* x, int x_dtype, size_t x_stride, const void* residual, size_t residual_stride, void* out, int out_dtype,
                size_t out_stride, size_t rows, size_t cols, const ft_dropout_t* drop, void* stream);
 

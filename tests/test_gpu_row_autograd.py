@@ -147,3 +147,15 @@ def test_gradient_of_a_gradient_penalty(cuda):
     g, = torch.autograd.grad((dropout(x, 0.5, 4).t() * w.t()).sum(), x, create_graph=True)
     got_w, = torch.autograd.grad(g.t().pow(2).sum(), w)
     assert torch.equal(got_w, want_w)
+
+
+def test_a_backward_pass_confined_to_some_leaves(cuda):
+    """``inputs=`` and ``torch.autograd.grad`` leave the accumulator alone, as they do a leaf that is not named."""
+    weight, acc = _randn(cuda, (20, 12), F32).requires_grad_(), torch.zeros((20, 12), device=cuda)
+    w = _randn(cuda, (12,), F32, 1).requires_grad_()
+    x = embedding(torch.arange(9, device=cuda), weight, grad_into=acc)
+    torch.autograd.grad((x * w).sum(), w, retain_graph=True)
+    (x * w).sum().backward(inputs=[w])
+    assert not bool(acc.any())
+    (x * w).sum().backward()
+    assert torch.equal(acc[:9], w.detach().expand(9, 12)) and not bool(acc[9:].any()) and weight.grad is None
